@@ -132,9 +132,7 @@ def _group_scales(x):
     """e8m0 bytes [NB, groups, HKV] of x [NB, HKV, block, D]: the smallest power of two that keeps a group's 16 rows within e4m3."""
     nb, hkv, block, _ = x.shape
     amax = x.reshape(nb, hkv, block // GROUP, GROUP * D).abs().amax(-1)
-    mant, exp = torch.frexp(amax / E4M3_MAX)
-    exp = torch.where(mant == 0.5, exp - 1, exp).clamp(min=SCALE_MIN_EXP)
-    return (exp + 127).to(torch.uint8).transpose(1, 2).contiguous()
+    return (_needed_exp(amax) + 127).to(torch.uint8).transpose(1, 2).contiguous()
 
 
 def _pool(g, nb, kv, block, kind):
@@ -254,9 +252,9 @@ def _codes(x):
 
 
 def _needed_exp(amax):
-    """Exponent of the smallest power of two s with amax / s <= 448."""
-    mant, exp = torch.frexp(amax / E4M3_MAX)
-    return torch.where(mant == 0.5, exp - 1, exp).clamp(min=SCALE_MIN_EXP)
+    """Exponent of the smallest power of two s >= 2^SCALE_MIN_EXP with amax / s <= 448."""
+    mant, exp = torch.frexp((amax / E4M3_MAX).clamp(min=2.0 ** SCALE_MIN_EXP))
+    return torch.where(mant == 0.5, exp - 1, exp)
 
 
 def _append_plain(s):
