@@ -17,6 +17,9 @@ _c_i64 = ctypes.c_int64
 _c_f = ctypes.c_float
 _c_sz = ctypes.c_size_t
 
+# The leading arguments of the rope_append entry points, up to `interleaved`.
+_ROPE_APPEND = [_c_vp, _c_i64] * 4 + [_c_vp] * 2 + [_c_i64] * 6 + [_c_vp, _c_vp, _c_i64, _c_i, _c_i64, _c_i, _c_i]
+
 # name -> (restype, argtypes).  Mirrors include/fp8kv_amd.h.
 SIGNATURES: dict[str, tuple] = {
     "fp8kv_status_string": (ctypes.c_char_p, [_c_i]),
@@ -59,6 +62,10 @@ SIGNATURES: dict[str, tuple] = {
     # fp8 KV-cache write (csrc/cache_write.hip)
     "fp8kv_cache_write": (_c_i, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp] + [_c_i64] * 6
                           + [_c_vp] * 3 + [_c_i] * 4 + [_c_vp]),
+    # position rotation and cache append in one pass (csrc/rope_append.hip)
+    "fp8kv_rope_append": (_c_i, _ROPE_APPEND + [_c_vp] * 3 + [_c_i] * 5 + [_c_i64, _c_vp]),
+    "fp8kv_rope_append_bf16": (_c_i, _ROPE_APPEND + [_c_vp] + [_c_i] * 5 + [_c_i64, _c_vp]),
+    "fp8kv_rope_append_blk": (_c_i, _ROPE_APPEND + [_c_vp] * 4 + [_c_i64] + [_c_i] * 7 + [_c_i64, _c_vp]),
     # layer epilogues (csrc/epilogues.hip, h4mv_silu_mul in csrc/h4mv.hip)
     "fp8kv_fused_add_rmsnorm": (_c_i, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_i, _c_i,
                                        _c_f, _c_i, _c_vp]),

@@ -368,6 +368,148 @@ def cache_write(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
     _lib.check("fp8kv_cache_write", st)
 
 
+# ------------------------------------------------------------------------------ rotation and cache append
+
+def rope_table(num_positions: int, rotary_dim: int, device, base: float = 10000.0,
+               dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """[num_positions, rotary_dim]: cos(p f_i), then sin(p f_i), f_i = base^(-2 i / rotary_dim), for
+    ``rope_append``.  Angles are formed in 64 bits (a product in 32 bits is off by 0.03 at position 10^6)
+    and rounded once.  Load-time helper: keep the table."""
+    if not (rotary_dim > 0 and rotary_dim % 2 == 0 and num_positions >= 0):
+        raise ValueError("rotary_dim must be even and positive, num_positions not negative")
+    freq = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
+    angle = torch.arange(num_positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], 1).to(dtype)
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _launch(name: str, t: torch.Tensor, *args) -> None:
+    """Entry point ``name`` on the current stream of ``t``'s device, whichever device is current."""
+    fn = getattr(_lib.load(), name)
+    if t.device.index == _current_device():
+        st = fn(*args, _stream_ptr(t))
+    else:
+        with torch.cuda.device(t.device):
+            st = fn(*args, _stream_ptr(t))
+    _lib.check(name, st)
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements between the token rows of [T, H, D] (a single row's stride says nothing)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _rope_args(q, key, value, k_cache, v_cache, positions, cos_sin, q_out, interleaved):
+    """Checks what the append calls share; (q_out, leading arguments of the C calls)."""
+    T, HKV, D = key.shape if key.dim() == 3 else (0, 0, 0)
+    for t, n in ((key, "key"), (value, "value")):
+        if not (t.is_cuda and t.dtype == torch.bfloat16 and t.dim() == 3 and t.shape == key.shape and
+                t.stride(2) == 1 and (t.stride(1) == D or HKV == 1)):
+            raise ValueError(f"{n} must be bf16 [T, HKV, D] with contiguous heads (key and value of one shape)")
+    dev = key.device
+    if not (k_cache.shape == v_cache.shape and k_cache.shape[2] == HKV and k_cache.shape[3] == D):
+        raise ValueError("caches must be [NB, PBLK, HKV, D] matching key")
+    if not (value.device == k_cache.device == v_cache.device == dev):
+        raise ValueError("tensors on different devices")
+    q_args = (None, 0, None, 0)
+    if q is not None:
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        for t, n in ((q, "q"), (q_out, "q_out")):
+            if not (t.dtype == torch.bfloat16 and t.dim() == 3 and t.device == dev and t.shape == q.shape and
+                    t.shape[0] == T and t.shape[2] == D and t.stride(2) == 1 and (t.stride(1) == D or t.shape[1] == 1)):
+                raise ValueError(f"{n} must be bf16 [T, HQ, D] with contiguous heads on key's device")
+        q_args = (q.data_ptr(), _row_stride(q), q_out.data_ptr(), _row_stride(q_out))
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    table = (None, None, 0, 0, 0, 0, 0)
+    if cos_sin is not None:
+        if not (cos_sin.dim() == 2 and cos_sin.dtype in (torch.float32, torch.bfloat16) and cos_sin.stride(1) == 1 and
+                cos_sin.device == dev):
+            raise ValueError("cos_sin must be fp32 or bf16 [positions, rotary_dim] on key's device")
+        if not (positions is not None and positions.dtype == torch.int64 and positions.shape == (T,) and
+                positions.is_contiguous() and positions.device == dev):
+            raise ValueError("positions must be a contiguous int64 device tensor [T]")
+        table = (positions.data_ptr(), cos_sin.data_ptr(), cos_sin.stride(0), int(cos_sin.dtype == torch.bfloat16),
+                 cos_sin.shape[0], cos_sin.shape[1], int(bool(interleaved)))
+    return q_out, (*q_args, key.data_ptr(), _row_stride(key), value.data_ptr(), _row_stride(value),
+                   k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+                   v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), *table)
+
+
+def rope_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
+                v_cache: torch.Tensor, positions: torch.Tensor | None, cos_sin: torch.Tensor | None,
+                slot_mapping: torch.Tensor, k_scale=None, v_scale=None, q_out: torch.Tensor | None = None,
+                interleaved: bool = False) -> torch.Tensor | None:
+    """Rotate ``q`` [T, HQ, D] into ``q_out`` (returned; may be ``q``), rotate ``key`` [T, HKV, D] and write
+    key and value at ``slot_mapping`` (as ``cache_write``; the slots distinct) of e4m3 caches with per-tensor
+    scales, or of bf16 caches, which ignore the scales.
+
+    ``cos_sin`` [positions, R] fp32 or bf16 holds cos then sin of every position's R / 2 angles
+    (``rope_table``); the first R elements of a head are rotated, paired in halves or, ``interleaved``,
+    adjacent.  A position outside the table gives NaN.  ``cos_sin=None``: no rotation; ``q=None``: keys and
+    values only.  fp32 arithmetic, rounded once (fp8kv_rope_append)."""
+    bf16_kv = _kv_caches_bf16(k_cache, v_cache)
+    q_out, args = _rope_args(q, key, value, k_cache, v_cache, positions, cos_sin, q_out, interleaved)
+    T, HKV, D = key.shape
+    dev = key.device
+    if not (slot_mapping.dtype == torch.int64 and slot_mapping.shape == (T,) and slot_mapping.is_contiguous() and
+            slot_mapping.device == dev):
+        raise ValueError("slot_mapping must be a contiguous int64 device tensor [T]")
+    if bf16_kv:
+        name, scales = "fp8kv_rope_append_bf16", ()
+    else:
+        if k_scale is None or v_scale is None:
+            raise ValueError("e4m3 caches need k_scale and v_scale")
+        ks, vs = _scale_tensor(k_scale, dev), _scale_tensor(v_scale, dev)
+        name, scales = "fp8kv_rope_append", (ks.data_ptr(), vs.data_ptr())
+    if T > 0:
+        _launch(name, key, *args, slot_mapping.data_ptr(), *scales, T, 0 if q is None else q.shape[1], HKV, D,
+                k_cache.shape[1], k_cache.shape[0])
+    return q_out
+
+
+def _kv_scales_check(kv_scales: torch.Tensor, k_cache: torch.Tensor) -> None:
+    NB, PBLK, HKV = k_cache.shape[:3]
+    if not (kv_scales.dtype in (torch.uint8, torch.float8_e8m0fnu) and kv_scales.device == k_cache.device and
+            kv_scales.shape == (NB, PBLK // 16, HKV, 2) and kv_scales.is_contiguous()):
+        raise ValueError(f"kv_scales must be contiguous uint8 (e8m0) [{NB}, {PBLK // 16}, {HKV}, 2] on the caches' device")
+
+
+def rope_append_blk(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
+                    v_cache: torch.Tensor, kv_scales: torch.Tensor, positions: torch.Tensor | None,
+                    cos_sin: torch.Tensor | None, query_start_loc: torch.Tensor, seq_lens: torch.Tensor,
+                    block_table: torch.Tensor, q_out: torch.Tensor | None = None,
+                    interleaved: bool = False) -> torch.Tensor | None:
+    """``rope_append`` into a block-scaled cache: e4m3 codes with a power-of-two scale per 16 tokens, kv
+    head and tensor, ``kv_scales`` [NB, PBLK / 16, HKV, 2] (e8m0 bytes of K and V).
+
+    The new tokens are the ends of the sequences: rows query_start_loc[s] .. query_start_loc[s + 1] - 1 are
+    the last tokens of sequence s, whose length with them is seq_lens[s] and whose blocks are block_table
+    row s (int32 device tensors, the metadata of the attention calls).  A group of 16 that also holds
+    earlier tokens keeps its scale unless the new ones need a larger one; then the old codes are re-rounded.
+    Rows of q_out behind the last sequence are left as they were (fp8kv_rope_append_blk)."""
+    _fp8_cache_check(k_cache, "k_cache")
+    _fp8_cache_check(v_cache, "v_cache")
+    q_out, args = _rope_args(q, key, value, k_cache, v_cache, positions, cos_sin, q_out, interleaved)
+    T, HKV, D = key.shape
+    dev = key.device
+    _kv_scales_check(kv_scales, k_cache)
+    for t, n in ((query_start_loc, "query_start_loc"), (seq_lens, "seq_lens"), (block_table, "block_table")):
+        if not (t.dtype == torch.int32 and t.device == dev and (t.stride(-1) == 1 or t.shape[-1] == 1)):
+            raise ValueError(f"{n} must be an int32 tensor on key's device, contiguous along its last axis")
+    if not (block_table.dim() == 2 and query_start_loc.shape == (block_table.shape[0] + 1,) and
+            seq_lens.shape == (block_table.shape[0],)):
+        raise ValueError("block_table must be [NS, max_blocks], query_start_loc [NS + 1], seq_lens [NS]")
+    if T > 0 and block_table.shape[0] > 0:
+        _launch("fp8kv_rope_append_blk", key, *args, kv_scales.data_ptr(), query_start_loc.data_ptr(),
+                seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+                block_table.shape[0], T, 0 if q is None else q.shape[1], HKV, D, k_cache.shape[1], k_cache.shape[0])
+    return q_out
+
+
 # ------------------------------------------------------------------------------ layer epilogues
 
 def _bf16_rows(t: torch.Tensor, name: str) -> None:

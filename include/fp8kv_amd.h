@@ -313,6 +313,77 @@ int fp8kv_cache_write(const void* key, int64_t key_row_stride,
                       void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Position rotation and KV-cache append in one pass: rotates queries, rotates new keys and writes
+ * keys and values into the paged cache.
+ *
+ *   rot(x, p): the first rotary_dim elements of a head in pairs (a, b) = (x[i], x[i + rotary_dim / 2]), or
+ *   (x[2 i], x[2 i + 1]) with interleaved != 0, i < rotary_dim / 2:
+ *     a' = a cos_sin[p][i] - b cos_sin[p][rotary_dim / 2 + i],  b' = b cos_sin[p][i] + a cos_sin[p][rotary_dim / 2 + i];
+ *   the other elements as they are.  fp32 arithmetic, one rounding at the end:
+ *     q_out[t] = bf16(rot(q[t], positions[t]))
+ *     k_cache[slot] = e4m3fn(rot(key[t], positions[t]) / k_scale), v_cache[slot] = e4m3fn(value[t] / v_scale)
+ *   (conversions as fp8kv_cache_write; bf16 caches: bf16(rot(key)), value).
+ *
+ *   q, q_out   bf16 [num_tokens, num_q_heads, head_size], row strides in elements (multiples of 8), heads
+ *              contiguous, 16-byte aligned; q_out may be q.  q NULL: no queries (num_q_heads ignored)
+ *   key, value bf16 [num_tokens, num_kv_heads, head_size] likewise
+ *   caches     as for fp8kv_cache_write (bf16: strides in elements, multiples of 8, 16-byte aligned)
+ *   positions  int64 [num_tokens]; cos_sin fp32 (cos_sin_bf16 == 0) or bf16 [num_positions, rotary_dim], row
+ *              stride in elements (a multiple of 4 or 8), 16-byte aligned.  cos_sin NULL: no rotation.
+ *              A position outside [0, num_positions) gives NaN in the rotated elements
+ *   slot_mapping int64 [num_tokens], the slots distinct; tokens whose slot is negative or past the cache's
+ *              num_blocks * block_size write no K and V (their queries are rotated all the same)
+ *   head_size % 16 == 0, rotary_dim % 16 == 0 and <= head_size, block_size a power of two.
+ *
+ * No counterpart in the reference, whose engine runs vLLM's rotary embedding and
+ * reshape_and_cache_flash (profiling/prof_h4mv.txt:9) as separate kernels. */
+int fp8kv_rope_append(const void* q, int64_t q_row_stride, void* q_out, int64_t q_out_row_stride,
+                      const void* key, int64_t key_row_stride, const void* value, int64_t value_row_stride,
+                      void* k_cache, void* v_cache,
+                      int64_t sk0, int64_t sk1, int64_t sk2, int64_t sv0, int64_t sv1, int64_t sv2,
+                      const int64_t* positions, const void* cos_sin, int64_t cos_sin_row_stride,
+                      int cos_sin_bf16, int64_t num_positions, int rotary_dim, int interleaved,
+                      const int64_t* slot_mapping, const float* k_scale, const float* v_scale,
+                      int num_tokens, int num_q_heads, int num_kv_heads, int head_size, int block_size,
+                      int64_t num_blocks, void* stream);
+
+int fp8kv_rope_append_bf16(const void* q, int64_t q_row_stride, void* q_out, int64_t q_out_row_stride,
+                           const void* key, int64_t key_row_stride, const void* value, int64_t value_row_stride,
+                           void* k_cache, void* v_cache,
+                           int64_t sk0, int64_t sk1, int64_t sk2, int64_t sv0, int64_t sv1, int64_t sv2,
+                           const int64_t* positions, const void* cos_sin, int64_t cos_sin_row_stride,
+                           int cos_sin_bf16, int64_t num_positions, int rotary_dim, int interleaved,
+                           const int64_t* slot_mapping,
+                           int num_tokens, int num_q_heads, int num_kv_heads, int head_size, int block_size,
+                           int64_t num_blocks, void* stream);
+
+/* The same into a block-scaled cache: e4m3 codes with one power-of-two scale per 16 tokens, kv head
+ * and tensor, kept as an e8m0 byte (2^(b - 127); 255 is NaN and never written):
+ *   kv_scales uint8 [num_blocks, block_size / 16, num_kv_heads, 2] contiguous (K byte, V byte); the 16 slots
+ *   16 j .. 16 j + 15 of block b form group (b, j), element = e4m3fn code * 2^(scale byte - 127).
+ * The tokens are those of whole sequences' ends, as in fp8kv_prefill_attn_varlen: sequence s owns rows
+ * query_start_loc[s] .. query_start_loc[s + 1] - 1 of q, key and value (int32 [num_seqs + 1], not
+ * descending), its last token is number seq_lens[s] - 1 (the new ones included), and block_table row s
+ * (max_blocks entries) maps it.  For each group that gets new tokens the exponent is the smallest e >= -100 with
+ * 2^e * 448 >= every finite |element| of its new rows, and not less than before where the group holds earlier tokens
+ * of the sequence; where it grows, their codes are re-rounded once.  Values are code = e4m3fn(x * 2^-e):
+ * infinities saturate, NaN stays NaN, and neither enters the scale.
+ * No other byte is touched: slots behind the last token, and rows of q_out from query_start_loc[num_seqs] on,
+ * stay as they were.  Tokens of negative number, columns from max_blocks on and block ids outside
+ * [0, num_blocks) are skipped.  No two sequences of a call may write to one block.
+ * head_size == 128, block_size a power of two >= 16. */
+int fp8kv_rope_append_blk(const void* q, int64_t q_row_stride, void* q_out, int64_t q_out_row_stride,
+                          const void* key, int64_t key_row_stride, const void* value, int64_t value_row_stride,
+                          void* k_cache, void* v_cache,
+                          int64_t sk0, int64_t sk1, int64_t sk2, int64_t sv0, int64_t sv1, int64_t sv2,
+                          const int64_t* positions, const void* cos_sin, int64_t cos_sin_row_stride,
+                          int cos_sin_bf16, int64_t num_positions, int rotary_dim, int interleaved,
+                          void* kv_scales, const int32_t* query_start_loc, const int32_t* seq_lens,
+                          const int32_t* block_table, int64_t bt_stride, int max_blocks, int num_seqs,
+                          int num_tokens, int num_q_heads, int num_kv_heads, int head_size, int block_size,
+                          int64_t num_blocks, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Layer epilogues around the MXFP4 linears (decode and prefill).
  *
  * The reference engine runs these as compiler-fused kernels of its vLLM model code (listed in
