@@ -63,20 +63,22 @@ __device__ __forceinline__ f32x2_t load_coherent2(const float* p)
 // vr[j] = bytes d = 8c .. 8c+7 of the group's k-slot j token (two e4m3 dwords).  The 8 x 8 byte
 // block is transposed in registers: each output dword pairs two tokens at one d (v_perm_b32), then
 // v_cvt_scalef32_pk_bf16_fp8 widens the byte pairs.  Fragment n (d row 8c + n) dword k is the bf16
-// pair (k-slot 2k, k-slot 2k + 1).
-__device__ __forceinline__ void v_fragments(const u32x2_t (&vr)[8], u32x4_t (&bf)[8])
+// pair (k-slot 2k, k-slot 2k + 1).  scale0 and scale1, powers of two, multiply k-slots 0-3 and 4-7 (the two
+// 16-token groups) on the way; the products are exact.
+__device__ __forceinline__ void v_fragments(const u32x2_t (&vr)[8], u32x4_t (&bf)[8], float scale0 = 1.0f, float scale1 = 1.0f)
 {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+        const float sc = k < 2 ? scale0 : scale1;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const uint32_t a = vr[2 * k][w], b = vr[2 * k + 1][w];
             const uint32_t x = __builtin_amdgcn_perm(b, a, 0x05010400u);   // a0 b0 a1 b1
             const uint32_t y = __builtin_amdgcn_perm(b, a, 0x07030602u);   // a2 b2 a3 b3
-            bf[4 * w + 0][k] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false));
-            bf[4 * w + 1][k] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true));
-            bf[4 * w + 2][k] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.0f, false));
-            bf[4 * w + 3][k] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, 1.0f, true));
+            bf[4 * w + 0][k] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, sc, false));
+            bf[4 * w + 1][k] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, sc, true));
+            bf[4 * w + 2][k] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, sc, false));
+            bf[4 * w + 3][k] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, sc, true));
         }
     }
 }

@@ -43,8 +43,10 @@
 #include "fp8kv_diag.h"
 #include "attn_common.h"
 #include "kv_chunk.h"
+#include "kv_visible.h"
 
 #include <mutex>
+#include <type_traits>
 
 namespace fp8kv {
 namespace decode_detail {
@@ -83,6 +85,12 @@ struct Params {
     int64_t sk0, sk1, sk2, sv0, sv1, sv2;
     float sm_scale;
     int hkv, gqa, pblk, pshift, nsplit;
+};
+
+// A call that sees part of the context (a window and the first tokens), or a block-scaled cache.
+struct VisibleParams : Params {
+    const uint16_t* kv_scales;      // block-scaled caches: [blocks][block_size / 16][hkv] pairs of e8m0 bytes
+    int window, sinks;
 };
 
 // Floats per split record, rounded up to a multiple of four so that every record starts 16-byte
@@ -154,11 +162,14 @@ __device__ __forceinline__ void merge_regs(const Params& P, const float* recs, i
 // preloading, so the hardware places them in SGPRs before the first instruction, and the sequence
 // length (the head of the dependent chain seq_lens -> block ids -> K/V) and the query row are
 // requested together with the rest of P instead of after it.
-// The kernel body, for e4m3 (B16 = false) or bf16 K/V caches.
-template <int W, int NG, int DEPTH, bool KF, bool B16>
+// The kernel body, for e4m3 or bf16 K/V caches over whole contexts (PT = Params), or for the visible keys of
+// any cache kind (PT = VisibleParams, kv_visible.h).
+template <int W, int NG, int DEPTH, bool KF, int KIND, typename PT>
 __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens, const int32_t* __restrict__ qsl,
-                                            const Params& P)
+                                            const PT& P)
 {
+    constexpr bool B16 = KIND == kBf16;
+    constexpr bool VISIBLE = std::is_same_v<PT, VisibleParams>;
     // The two loads go out together with the loads of every argument the block-id, Q and K/V
     // requests need (the asm takes all of them, so one wait covers them all) rather than after
     // them; later reads of these fields reuse the loaded values.
@@ -194,7 +205,18 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
     const int gqa = P.gqa;
 
     int lo, hi;
-    split_span(seqlen, nsplit, sp, lo, hi);
+    [[maybe_unused]] Walk walk;
+    if constexpr (VISIBLE) {
+        walk = make_walk(seqlen, P.window, P.sinks);
+        split_span(walk.nv, nsplit, sp, lo, hi);
+    } else {
+        split_span(seqlen, nsplit, sp, lo, hi);
+    }
+    // The three steps of a chunk: its block ids, its loads, its use.
+    auto ids_of = [&](const int32_t* row, int c0, int end) {
+        if constexpr (VISIBLE) return load_chunk_ids<NG>(P, row, c0, end, walk);
+        else return load_chunk_ids<NG>(P, row, c0, end);
+    };
     const int32_t* btrow = bt + (int64_t)seq * bt_stride;
 
     // The wave's chunks start at c_first and step by `stride`.
@@ -206,8 +228,8 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
     [[maybe_unused]] ChunkIds<NG> ia, ib;
     if constexpr (DEPTH != 1) {
         if (c_first < hi) {
-            ia = load_chunk_ids<NG>(P, btrow, c_first, last);
-            ib = load_chunk_ids<NG>(P, btrow, c_first + stride, last);
+            ia = ids_of(btrow, c_first, last);
+            ib = ids_of(btrow, c_first + stride, last);
         }
     }
 
@@ -223,9 +245,9 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
         qf[2] = load_16(qrow + 64 + 16 * lp);
         qf[3] = load_16(qrow + 64 + 16 * lp + 8);
     }
-    // bf16 caches carry no scales (the reference ignores k_scale and v_scale for them).
-    const float qk_scale = B16 ? P.sm_scale * kLog2e : P.sm_scale * *(const_f32_t*)P.k_scale * kLog2e;
-    const float vs = B16 ? 1.f : *(const_f32_t*)P.v_scale;
+    // bf16 caches carry no scales (the reference ignores k_scale and v_scale for them), block-scaled ones their own.
+    const float qk_scale = KIND != kE4m3 ? P.sm_scale * kLog2e : P.sm_scale * *(const_f32_t*)P.k_scale * kLog2e;
+    const float vs = KIND != kE4m3 ? 1.f : *(const_f32_t*)P.v_scale;
 
     WaveState st;
     st.m_run = neg_inf();
@@ -237,12 +259,22 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
         const LaneOffsets lofs = lane_offsets<B16>(P, lr, lp);
         ChunkRegs<NG, B16> ca;
         [[maybe_unused]] ChunkRegs<NG, B16> cb;
+        [[maybe_unused]] ChunkScales<NG> sa, sb;
+        auto issue = [&](ChunkRegs<NG, B16>& c, ChunkScales<NG>& sc, const ChunkIds<NG>& ids, int at) {
+            if constexpr (KIND == kBlk) issue_scales<NG>(sc, P, ids, kh, at, last, walk);
+            if constexpr (VISIBLE) issue_chunk<NG, KF, B16>(c, P, lofs, ids, kh, at, hi, last, walk);
+            else issue_chunk<NG, KF, B16>(c, P, lofs, ids, kh, at, hi, last);
+        };
+        auto consume = [&](const ChunkRegs<NG, B16>& c, const ChunkScales<NG>& sc, int at) {
+            if constexpr (VISIBLE) consume_visible<NG, KIND>(c, sc, st, qf, qk_scale, at, hi, walk, lp);
+            else consume_chunk<NG, B16>(c, st, qf, qk_scale, at, hi - 1, at + CH > hi, hi, lp);
+        };
         int c0 = c_first;
         if constexpr (DEPTH == 1) {
             do {
-                const ChunkIds<NG> ia = load_chunk_ids<NG>(P, btrow, c0, last);
-                issue_chunk<NG, KF, B16>(ca, P, lofs, ia, kh, c0, hi, last);
-                consume_chunk<NG, B16>(ca, st, qf, qk_scale, c0, hi - 1, c0 + CH > hi, hi, lp);
+                const ChunkIds<NG> ia = ids_of(btrow, c0, last);
+                issue(ca, sa, ia, c0);
+                consume(ca, sa, c0);
                 c0 += stride;
             } while (c0 < hi);
         } else {
@@ -252,15 +284,15 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
             // reads one broadcast line per instruction and is not used.
             do {
                 ids_ready(ia, ib);
-                issue_chunk<NG, KF, B16>(ca, P, lofs, ia, kh, c0, hi, last);
-                issue_chunk<NG, KF, B16>(cb, P, lofs, ib, kh, c0 + stride, hi, last);
+                issue(ca, sa, ia, c0);
+                issue(cb, sb, ib, c0 + stride);
                 if (c0 + 2 * stride < hi) {            // the next pair's ids, a round trip ahead
-                    ia = load_chunk_ids<NG>(P, btrow, c0 + 2 * stride, last);
-                    ib = load_chunk_ids<NG>(P, btrow, c0 + 3 * stride, last);
+                    ia = ids_of(btrow, c0 + 2 * stride, last);
+                    ib = ids_of(btrow, c0 + 3 * stride, last);
                 }
-                consume_chunk<NG, B16>(ca, st, qf, qk_scale, c0, hi - 1, c0 + CH > hi, hi, lp);
+                consume(ca, sa, c0);
                 if (c0 + stride >= hi) break;
-                consume_chunk<NG, B16>(cb, st, qf, qk_scale, c0 + stride, hi - 1, c0 + stride + CH > hi, hi, lp);
+                consume(cb, sb, c0 + stride);
                 c0 += 2 * stride;
             } while (c0 < hi);
         }
@@ -438,7 +470,7 @@ template <int W, int NG, int DEPTH, bool KF>
 __global__ void __launch_bounds__(W * 64)
 decode_kernel(const int32_t* __restrict__ seq_lens, const int32_t* __restrict__ qsl, Params P)
 {
-    decode_body<W, NG, DEPTH, KF, false>(seq_lens, qsl, P);
+    decode_body<W, NG, DEPTH, KF, kE4m3>(seq_lens, qsl, P);
 }
 
 // bf16 K/V caches: the same kernel with twice the bytes per chunk and no widening (the reference's
@@ -447,7 +479,15 @@ template <int W, int NG, int DEPTH, bool KF>
 __global__ void __launch_bounds__(W * 64)
 decode_bf16kv_kernel(const int32_t* __restrict__ seq_lens, const int32_t* __restrict__ qsl, Params P)
 {
-    decode_body<W, NG, DEPTH, KF, true>(seq_lens, qsl, P);
+    decode_body<W, NG, DEPTH, KF, kBf16>(seq_lens, qsl, P);
+}
+
+// The visible keys of a window and the first tokens, over caches of any kind, and block-scaled caches whole.
+template <int W, int NG, int DEPTH, bool KF, int KIND>
+__global__ void __launch_bounds__(W * 64)
+decode_visible_kernel(const int32_t* __restrict__ seq_lens, const int32_t* __restrict__ qsl, VisibleParams P)
+{
+    decode_body<W, NG, DEPTH, KF, KIND>(seq_lens, qsl, P);
 }
 
 inline size_t counters_bytes() { return (size_t)kMaxPairs * sizeof(uint32_t); }
@@ -689,6 +729,29 @@ int decode_launch(const Params& P, int num_seqs, int max_seq_len, hipStream_t st
     return finish_launch();
 }
 
+// Longest visible set of a call (kv_visible.h): what its splits and their launch go by.  0: not known.
+inline int visible_len(int max_seq_len, int window, int sinks)
+{
+    if (window <= 0) return max_seq_len;
+    const int64_t most = (int64_t)window + sinks;
+    return max_seq_len <= 0 || max_seq_len > most ? (int)(most < kUnknownContext ? most : kUnknownContext) : max_seq_len;
+}
+
+template <int KIND>
+int launch_visible(const VisibleParams& P, int num_seqs, int max_seq_len, hipStream_t st)
+{
+    const dim3 grid((unsigned)P.nsplit, (unsigned)P.hkv, (unsigned)num_seqs), block(8 * 64);
+    begin_launch();
+    if constexpr (KIND == kBf16) {
+        launch_kernel(decode_visible_kernel<8, 2, 2, true, KIND>, grid, block, 0, st, P.seq_lens, P.qsl, P);
+    } else if (pick_variant((int64_t)P.nsplit * P.hkv * num_seqs, P.nsplit, visible_len(max_seq_len, P.window, P.sinks)) == 1) {
+        launch_kernel(decode_visible_kernel<8, 2, 1, false, KIND>, grid, block, 0, st, P.seq_lens, P.qsl, P);
+    } else {
+        launch_kernel(decode_visible_kernel<8, 2, 2, false, KIND>, grid, block, 0, st, P.seq_lens, P.qsl, P);
+    }
+    return finish_launch();
+}
+
 }  // namespace decode_detail
 }  // namespace fp8kv
 
@@ -870,4 +933,84 @@ extern "C" void fp8kv_decode_tune(int variant, int target_wgs)
 extern "C" int fp8kv_decode_variant(int num_seqs, int num_kv_heads, int num_splits, int max_seq_len)
 {
     return pick_variant((int64_t)num_seqs * num_kv_heads * num_splits, num_splits, max_seq_len);
+}
+
+namespace fp8kv {
+namespace decode_detail {
+
+// What the three entry points below share.
+template <int KIND>
+int decode_visible(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache, int64_t sk0, int64_t sk1,
+                   int64_t sk2, int64_t sv0, int64_t sv1, int64_t sv2, void* out, int64_t out_row_stride,
+                   const int32_t* query_start_loc, const int32_t* seq_lens, const int32_t* block_table, int64_t bt_stride,
+                   const float* k_scale, const float* v_scale, const void* kv_scales, float sm_scale, int num_seqs,
+                   int num_q_heads, int num_kv_heads, int head_size, int block_size, int num_splits, void* scratch_buf,
+                   size_t scratch_bytes_given, int window, int sinks, int max_seq_len, void* stream)
+{
+    if (window < 0 || sinks < 0) return FP8KV_ERR_ARG;
+    if (KIND == kE4m3 && (!k_scale || !v_scale)) return FP8KV_ERR_ARG;
+    if (KIND == kBlk && !kv_scales) return FP8KV_ERR_ARG;
+    VisibleParams P;
+    size_t need = 0;
+    const float* unused = reinterpret_cast<const float*>(q);        // scales that only the kE4m3 kernel reads
+    const int rc = decode_setup(P, q, q_row_stride, k_cache, v_cache, sk0, sk1, sk2, sv0, sv1, sv2, out, out_row_stride,
+                                query_start_loc, seq_lens, block_table, bt_stride, KIND == kE4m3 ? k_scale : unused,
+                                KIND == kE4m3 ? v_scale : unused, sm_scale, num_seqs, num_q_heads, num_kv_heads, head_size,
+                                block_size, num_splits, need, KIND == kBf16 ? 2 : 1);
+    if (rc != FP8KV_OK) return rc;
+    if (KIND == kBlk && !aligned(kv_scales, 2)) return FP8KV_ERR_ALIGN;
+    if (need > 0 && (!scratch_buf || scratch_bytes_given < need || !aligned(scratch_buf, 256)))
+        return FP8KV_ERR_SCRATCH;
+    use_scratch(P, scratch_buf, need);
+    P.kv_scales = static_cast<const uint16_t*>(kv_scales);
+    P.window = window;
+    P.sinks = sinks;
+    return launch_visible<KIND>(P, num_seqs, max_seq_len, reinterpret_cast<hipStream_t>(stream));
+}
+
+}  // namespace decode_detail
+}  // namespace fp8kv
+
+extern "C" int fp8kv_decode_attn_window(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                        int64_t sk0, int64_t sk1, int64_t sk2, int64_t sv0, int64_t sv1, int64_t sv2,
+                                        void* out, int64_t out_row_stride, const int32_t* query_start_loc,
+                                        const int32_t* seq_lens, const int32_t* block_table, int64_t bt_stride,
+                                        const float* k_scale, const float* v_scale, float sm_scale, int num_seqs,
+                                        int num_q_heads, int num_kv_heads, int head_size, int block_size, int num_splits,
+                                        void* scratch_buf, size_t scratch_bytes_given, int window, int sinks,
+                                        int max_seq_len, void* stream)
+{
+    return decode_visible<kE4m3>(q, q_row_stride, k_cache, v_cache, sk0, sk1, sk2, sv0, sv1, sv2, out, out_row_stride,
+                                 query_start_loc, seq_lens, block_table, bt_stride, k_scale, v_scale, nullptr, sm_scale,
+                                 num_seqs, num_q_heads, num_kv_heads, head_size, block_size, num_splits, scratch_buf,
+                                 scratch_bytes_given, window, sinks, max_seq_len, stream);
+}
+
+extern "C" int fp8kv_decode_attn_window_bf16(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                             int64_t sk0, int64_t sk1, int64_t sk2, int64_t sv0, int64_t sv1, int64_t sv2,
+                                             void* out, int64_t out_row_stride, const int32_t* query_start_loc,
+                                             const int32_t* seq_lens, const int32_t* block_table, int64_t bt_stride,
+                                             float sm_scale, int num_seqs, int num_q_heads, int num_kv_heads,
+                                             int head_size, int block_size, int num_splits, void* scratch_buf,
+                                             size_t scratch_bytes_given, int window, int sinks, int max_seq_len,
+                                             void* stream)
+{
+    return decode_visible<kBf16>(q, q_row_stride, k_cache, v_cache, sk0, sk1, sk2, sv0, sv1, sv2, out, out_row_stride,
+                                 query_start_loc, seq_lens, block_table, bt_stride, nullptr, nullptr, nullptr, sm_scale,
+                                 num_seqs, num_q_heads, num_kv_heads, head_size, block_size, num_splits, scratch_buf,
+                                 scratch_bytes_given, window, sinks, max_seq_len, stream);
+}
+
+extern "C" int fp8kv_decode_attn_blk(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                     int64_t sk0, int64_t sk1, int64_t sk2, int64_t sv0, int64_t sv1, int64_t sv2,
+                                     void* out, int64_t out_row_stride, const int32_t* query_start_loc,
+                                     const int32_t* seq_lens, const int32_t* block_table, int64_t bt_stride,
+                                     const void* kv_scales, float sm_scale, int num_seqs, int num_q_heads,
+                                     int num_kv_heads, int head_size, int block_size, int num_splits, void* scratch_buf,
+                                     size_t scratch_bytes_given, int window, int sinks, int max_seq_len, void* stream)
+{
+    return decode_visible<kBlk>(q, q_row_stride, k_cache, v_cache, sk0, sk1, sk2, sv0, sv1, sv2, out, out_row_stride,
+                                query_start_loc, seq_lens, block_table, bt_stride, nullptr, nullptr, kv_scales, sm_scale,
+                                num_seqs, num_q_heads, num_kv_heads, head_size, block_size, num_splits, scratch_buf,
+                                scratch_bytes_given, window, sinks, max_seq_len, stream);
 }

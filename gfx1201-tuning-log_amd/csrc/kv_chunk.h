@@ -42,8 +42,15 @@ struct ChunkIds {
 typedef __attribute__((address_space(4))) const int32_t const_i32_t;   // read-only for the launch
 typedef __attribute__((address_space(4))) const float const_f32_t;
 
-template <int NG, typename PT>
-__device__ __forceinline__ ChunkIds<NG> load_chunk_ids(const PT& P, const int32_t* btrow, int c0, int last)
+// Where a 16-token group of the walked tokens starts in its sequence: as walked, unless the caller leaves
+// tokens out.
+struct WalkAll {
+    __device__ __forceinline__ int operator()(int t0) const { return t0; }
+};
+
+template <int NG, typename PT, typename Place = WalkAll>
+__device__ __forceinline__ ChunkIds<NG> load_chunk_ids(const PT& P, const int32_t* btrow, int c0, int last,
+                                                       const Place& place = Place())
 {
     // The constant address space makes the compiler use scalar loads for these uniform reads,
     // whatever stores or fences come before them in the kernel.
@@ -52,7 +59,7 @@ __device__ __forceinline__ ChunkIds<NG> load_chunk_ids(const PT& P, const int32_
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         const int t0 = c0 + 16 * g;
-        ids.blk[g] = row[(t0 < last ? t0 : last) >> P.pshift];
+        ids.blk[g] = row[place(t0 < last ? t0 : last) >> P.pshift];
     }
     return ids;
 }
@@ -98,13 +105,14 @@ __device__ __forceinline__ LaneOffsets lane_offsets(const PT& P, int lr, int lp)
 // base address is scalar (block id from `ids`), the per-lane part a 32-bit offset.  KF requests
 // the K bytes of every group before any V byte, so the S^T MFMAs and the softmax of a chunk can
 // start while its V bytes are still arriving; otherwise K and V alternate per group.
-template <int NG, bool KF, bool B16, typename PT>
+template <int NG, bool KF, bool B16, typename PT, typename Place = WalkAll>
 __device__ __forceinline__ void issue_chunk(ChunkRegs<NG, B16>& c, const PT& P, const LaneOffsets& lo_,
-                                            const ChunkIds<NG>& ids, int kh, int c0, int hi, int last)
+                                            const ChunkIds<NG>& ids, int kh, int c0, int hi, int last,
+                                            const Place& place = Place())
 {
     auto slot_of = [&](int g) -> int64_t {
         const int t0 = c0 + 16 * g;
-        return (int64_t)((t0 < last ? t0 : last) & (P.pblk - 1));
+        return (int64_t)(place(t0 < last ? t0 : last) & (P.pblk - 1));
     };
     auto issue_k = [&](int g) {
         const uint32_t m = c0 + 16 * g < hi ? ~0u : 0u;

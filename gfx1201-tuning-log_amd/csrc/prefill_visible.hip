@@ -1,0 +1,866 @@
+// Causal prefill attention over the visible keys of each query (a sliding window and the first tokens, or
+// everything before it), on e4m3 caches with one scale per tensor, block-scaled e4m3 caches and bf16
+// caches, for gfx950.
+//
+// Mathematics.  Query i of a sequence is token p = seq_len - qlen + i.  It sees the keys t <= p with
+// t > p - window or t < sinks (window 0: all t <= p), and with g(t) the 16-token group of t
+//   out = sum_t w_t 2^ev(g) V_t / sum_t w_t,   w_t = exp(sm_scale (q . 2^ek(g) K_t) - max)
+// (per-tensor scales: k_scale joins sm_scale and v_scale the result; bf16: no scales).  Rows that see
+// nothing (p < 0) are zeros.
+//
+// What bounds it: the matrix units and the softmax's exponentials; the keys of a token block are read
+// from L2 by its workgroup alone.  The shape is the key-split one of prefill_attn.hip: a workgroup of 8 waves
+// owns 16 tokens (MB: 4 / GQA blocks of them) of one kv head's query heads, or a pair of such blocks where
+// all of a causal context is seen; wave w takes row-set group w / NR, RS sets of 16 (token, head) rows,
+// and of every ring window the key tiles of residue w % NR.  Raw rows stream through an LDS ring of two windows.  Here:
+//   * a block walks the 32-key tiles that hold a visible key: those of the sinks, then those from
+//     the first query's window on.  A 16-key group inside them that holds none is not read (nor its
+//     block-table entry): its rows are copied from the window's first group and masked.
+//   * masks are applied only on tiles that some row of the block does not see whole.
+//   * e4m3 V enters P.V in fp16, where codes are exact, and so do the weights: they keep 11 bits instead of bf16's 8
+//     and are at most 2^kRescaleSlack.  bf16 V stays bf16, and so do its weights; their sum is then taken of
+//     the rounded values, so that the weights add up to one.
+//   * block scales (SC) are powers of two.  K's byte is the A scale of the block-scaled MFMA that forms the scores
+//     anyway.  V's multiplies the weights, whose products with it are kept in range row by row: the accumulators
+//     of a row are in units of 2^e (e_run), where e + m follows the row's running maximum of log2 w + ev
+//     like m follows that of log2 w, so a row's precision goes by the keys that it sees and weighs, not by its
+//     neighbours' scales.  A group's pair of bytes is loaded with the window's copies and passed through LDS.
+//   * a masked key's V must not reach a row through 0 * NaN: on masked tiles that hold a non-finite V
+//     (one test of the raw words), it is zeroed for the product and added afterwards to the rows that see it.
+#include "fp8kv_common.h"
+#include "fp8kv_status.h"
+#include "attn_common.h"
+#include "prefill_tiles.h"
+
+namespace fp8kv {
+namespace prefill_detail {
+
+struct VisibleParams : Params {
+    const uint16_t* kv_scales;      // [blocks][block_size / 16][hkv] pairs of e8m0 bytes (K low), or null
+    int window, sinks;
+};
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x4_t mfma16x16x32_f16(u32x4_t a, u32x4_t b, f32x4_t c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
+}
+
+// Scores of one 16-key group: K codes times the group's scale (byte KG * 2 of `scales`) against a split
+// query row.
+template <int KG, bool LO>
+__device__ __forceinline__ f32x4_t score_mfma(const v8i& k, const v8i& q, f32x4_t c, uint32_t scales)
+{
+    constexpr int qs = 127 | (127 + kQLoExp) << 8;
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q, c, 0, 0, 2 * KG, (int)scales, LO ? 1 : 0, qs);
+}
+
+__device__ __forceinline__ uint32_t f16x2_bits(f16x2_t v) { return __builtin_bit_cast(uint32_t, v); }
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b)
+{
+    f16x2_t v;
+    v[0] = (_Float16)a;
+    v[1] = (_Float16)b;
+    return f16x2_bits(v);
+}
+
+// Any non-finite element among the e4m3 codes (bf16 values) of a word.
+template <bool B16>
+__device__ __forceinline__ uint32_t non_finite(uint32_t w)
+{
+    return B16 ? ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u : ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+}
+// The word with its non-finite elements zeroed.
+template <bool B16>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w)
+{
+    const uint32_t bad = non_finite<B16>(w);          // the top bit of each bad element's field
+    const uint32_t mask = B16 ? (bad << 1) - (bad >> 15) : (bad << 1) - (bad >> 7);
+    return w & ~mask;
+}
+
+// rescale_rows for block-scaled V: ev[g] is the exponent of group g's scale, e_run the row's unit of o in log2.
+template <int RS>
+__device__ __forceinline__ void rescale_rows_scaled(f32x4_t (&sc)[RS][2], float (&m_run)[RS], float (&l_run)[RS],
+                                                    f32x4_t (&o)[RS][8], const float (&qkr)[RS], float (&e_run)[RS],
+                                                    const float (&ev)[2])
+{
+    auto group_max = [&](int j, int g) {
+        return max_raw(max3_raw(sc[j][g][0], sc[j][g][1], sc[j][g][2]), sc[j][g][3]);
+    };
+    bool any_need = false;
+#pragma unroll
+    for (int j = 0; j < RS; ++j) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const float x = group_max(j, g) * qkr[j] - m_run[j];
+            any_need |= x > kRescaleSlack || x + ev[g] > e_run[j] + kRescaleSlack;
+        }
+    }
+    if (__any(any_need)) {
+#pragma unroll
+        for (int j = 0; j < RS; ++j) {
+            // opaque: the maxima are formed again instead of being held over the test
+            asm volatile("" : "+v"(sc[j][0][0]), "+v"(sc[j][1][0]));
+            const float m0 = max_xor16_32_raw(group_max(j, 0)) * qkr[j], m1 = max_xor16_32_raw(group_max(j, 1)) * qkr[j];
+            const float mc = max_raw(m0, m1);                      // -inf for a fully masked row
+            const float m_new = mc > m_run[j] + kRescaleSlack ? mc : m_run[j];
+            const float down = m_run[j] - m_new;
+            const float top = max_raw((m0 - m_new) + ev[0], (m1 - m_new) + ev[1]);
+            const bool need = down < 0.f || top > e_run[j] + kRescaleSlack;
+            const float e_new = need ? max_raw(e_run[j] + down, top) : e_run[j];
+            const float alpha = __builtin_amdgcn_exp2f(down + (e_run[j] - e_new));
+            l_run[j] *= __builtin_amdgcn_exp2f(down);
+#pragma unroll
+            for (int n = 0; n < 8; ++n) o[j][n] *= alpha;
+            m_run[j] = m_new;
+            e_run[j] = e_new;
+        }
+    }
+}
+
+// SC: block-scaled e4m3 caches.
+template <int RS, int NG, int TPW, bool B16, bool MB, bool SC>
+__global__ void __launch_bounds__(kSplitWaves * 64)
+prefill_visible_kernel(VisibleParams P)
+{
+    constexpr int W = kSplitWaves;
+    constexpr int TILE = B16 ? kTileBytes16 : kTileBytes;
+    constexpr int NR = W / NG;
+    constexpr int NT = NR * TPW;                           // tiles per window
+    constexpr bool HALVES = SC && RS > 2;                  // V widened in two halves: no registers for both at once
+    static_assert(NG * NR == W && RS >= 1 && NT <= 64, "split shape");
+    constexpr int kWinBytes = NT * TILE;
+    constexpr int kRingBytes = 2 * kWinBytes;
+    constexpr int kStageBytes = NG * RS * (NR - 1) * kStageFloats * 4;
+    // the query rows' hand-over: the ring's second window, or behind the ring where that is too small
+    constexpr int kSetBytes = 4 * 1024 + 256;
+    constexpr int kExch = NG * RS * kSetBytes <= kWinBytes ? kWinBytes : kRingBytes;
+    constexpr int kExchEnd = B16 ? 0 : kExch + NG * RS * kSetBytes;
+    constexpr int kLoopBytes = kRingBytes > kExchEnd ? kRingBytes : kExchEnd;
+    __shared__ __align__(16) unsigned char ring[kLoopBytes > kStageBytes ? kLoopBytes : kStageBytes];
+    __shared__ float stage_m[NR > 1 ? NG * NR * RS * 16 : 4];
+    static_assert(!(B16 && SC), "block scales belong to e4m3 caches");
+    __shared__ __align__(4) uint16_t lds_scales[2][SC ? NT : 1][2];
+    float* const stage = reinterpret_cast<float*>(ring);
+
+    const int lin = blockIdx.x, seq = blockIdx.z;
+    int kh, rank;
+    if (P.xcd_map) {
+        const int xcd = lin & 7, per = 8 / P.hkv;
+        kh = xcd % P.hkv;
+        rank = (lin >> 3) * per + xcd / P.hkv;
+    } else {
+        kh = lin % P.hkv;
+        rank = lin / P.hkv;
+    }
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = wave / NR;
+    const int res = wave % NR;
+    const int lr = lane & 15;
+    const int lp = lane >> 4;
+
+    const int q_begin = P.cu_q[seq], qlen = P.cu_q[seq + 1] - q_begin;
+    const int q0 = P.seq_lens[seq] - qlen;                         // may be negative: those rows see nothing
+    const int nbt = MB ? P.nb : 1;                                 // token blocks of 16 per workgroup
+    const int n16 = (qlen + 16 * nbt - 1) / (16 * nbt);
+    const int tb = P.ntb_grid - 1 - rank;
+    const int nwg = P.paired ? (n16 + 1) >> 1 : n16;              // workgroups this sequence needs
+    if (tb < 0 || tb >= nwg) return;                              // whole workgroup, before any barrier
+    const int blk_a = tb, blk_b = P.paired ? n16 - 1 - tb : tb;
+    const int nphase = blk_b > blk_a ? 2 : 1;
+    const int32_t* btrow = P.bt + (int64_t)seq * P.bt_stride;
+    const float qk_signed = B16 || SC ? P.sm_scale * kLog2e : P.sm_scale * P.k_scale[0] * kLog2e;
+    auto uniform = [](float f) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(f))); };
+    const float qk = uniform(fabsf(qk_signed));                // a NaN reaches the output through vs
+    const uint32_t qflip = qk_signed < 0.f ? (B16 ? 0x80008000u : 0x80808080u) : 0u;   // negate Q (exact)
+    const float vs = uniform((B16 || SC ? 1.f : P.v_scale[0]) + (qk_signed == qk_signed ? 0.f : qk_signed));
+    const int window = P.window > 0 ? P.window : 1 << 30;
+    const int sinks = P.sinks;
+
+    // This wave's copies of every tile, lane (row, chunk), as in prefill_attn.hip: e4m3 one, of K rows (waves 0-3)
+    // or V rows (waves 4-7) 8 (wave & 3) .. +7; bf16 two, of K and V rows 4 wave .. +3.  Its rows lie in one
+    // 16-key group, hence in one cache block.
+    const bool dma_v = !B16 && wave >= 4;
+    int dma_r, dma_c;
+    if constexpr (B16) {
+        dma_r = lane >> 4;
+        dma_c = (lane & 15) ^ ((4 * wave + dma_r) & 15);
+    } else {
+        dma_lane_rc(dma_v, lane, dma_r, dma_c);
+    }
+    const int dma_row0 = B16 ? 4 * wave : 8 * (wave & 3);
+    const uint8_t* dma_base = dma_v ? P.v + (int64_t)kh * P.sv2 : P.k + (int64_t)kh * P.sk2;
+    const int64_t dma_s0 = dma_v ? P.sv0 : P.sk0;
+    const uint32_t dma_s1 = (uint32_t)(dma_v ? P.sv1 : P.sk1);    // < 2^32 / block size (host check)
+    const uint32_t dma_chunk = 16u * (uint32_t)dma_c;
+    const uint32_t voff_lane = (uint32_t)dma_r * dma_s1 + dma_chunk;
+    const uint8_t* const dma_base_v = P.v + (int64_t)kh * P.sv2;   // bf16: the second copy
+    const uint32_t voff_lane_v = (uint32_t)dma_r * (uint32_t)P.sv1 + dma_chunk;
+
+    // head, and block within the workgroup, of row-set rset (those past the last repeat it)
+    auto head_of = [&](int rset) {
+        rset = min(rset, nbt * P.gqa - 1);
+        return MB ? rset % P.gqa : rset;
+    };
+    auto block_of = [&](int rset) { return MB ? min(rset, nbt * P.gqa - 1) / P.gqa : 0; };
+
+    for (int ph = 0; ph < nphase; ++ph) {
+        const int blk = ph == 0 ? blk_b : blk_a;
+        const int tok0 = 16 * nbt * blk;                          // first token of the block(s)
+        const int qfirst = q0 + tok0;
+        const int qlast = q0 + min(tok0 + 16 * nbt, qlen) - 1;
+        const int k_hi = max(qlast + 1, 0);                       // keys [0, k_hi)
+        // Tiles walked: `head` ones that hold sinks, then, `jump` further, those from the window of the first query on.
+        const int low = max(qfirst - window + 1, 0);              // first key of that window
+        const int head = (min(sinks, low) + kBN - 1) / kBN;
+        const int jump = max(low / kBN - head, 0);
+        const int ntiles = (k_hi + kBN - 1) / kBN - jump;
+        const int nwin = (ntiles + NT - 1) / NT;
+        const int first_group = low >> 4;
+        auto tile_at = [&](int t) { return t + (t >= head ? jump : 0); };
+        // First key that this wave's copy of walked tile t reads: of its own group, or of the window's first
+        // where nobody sees a key of its own.
+        auto copy_key = [&](int t) {
+            const int row = kBN * tile_at(t) + dma_row0;
+            const int g = row >> 4;
+            return g >= first_group || 16 * g < sinks ? row : 16 * first_group + (dma_row0 & 15);
+        };
+        auto token_of = [&](int j) { return tok0 + 16 * block_of(grp * RS + j) + lr; };
+        // Several blocks: keys past this wave's last row, and below its first row's window, are left out.
+        const int my_hi = MB ? qfirst + 16 * block_of(grp * RS + RS - 1) + 15 : k_hi;
+        const int my_low = MB ? qfirst + 16 * block_of(grp * RS) - window + 1 : 0;
+
+        // Block ids for this wave's copy of each tile of window wi: lane u holds that of its tile u.
+        int bids = 0;
+        auto load_bids = [&](int wi) {
+            const int key0 = min(copy_key(wi * NT + lane), k_hi - 1);
+            bids = lane < NT ? btrow[key0 >> P.pshift] : 0;
+        };
+        // Scale bytes of window wi's groups, by the two waves whose K copies cover a tile's groups (rows 0 and 16): lane u
+        // those of tile u.  Follows load_bids(wi).
+        [[maybe_unused]] uint32_t sc_next = 0;
+        auto load_scales = [&](int wi) {
+            if constexpr (SC) {
+                if ((wave == 0 || wave == 2) && lane < NT) {
+                    const int key0 = min(copy_key(wi * NT + lane), k_hi - 1);
+                    sc_next = P.kv_scales[((int64_t)bids * (P.pblk >> 4) + ((key0 & (P.pblk - 1)) >> 4)) * P.hkv + kh];
+                }
+            }
+        };
+        // Copies of tiles u0 .. u1 - 1 of window wi (keys >= k_hi fetch key k_hi - 1; the causal mask removes them).
+        auto issue_window = [&](int wi, int u0, int u1) {
+#pragma unroll
+            for (int u = u0; u < u1; ++u) {
+                const int t = wi * NT + u;
+                if (t < ntiles) {
+                    const int64_t b = __builtin_amdgcn_readlane(bids, u);
+                    const uint8_t* sb = dma_base + b * dma_s0;
+                    const uint8_t* sbv = dma_base_v + b * P.sv0;
+                    uint32_t voff = voff_lane, voff_v = voff_lane_v;
+                    const int key = copy_key(t);
+                    if (key + 16 > k_hi) {                  // near the end of the keys
+                        const uint32_t slot = (uint32_t)(min(key + dma_r, k_hi - 1) & (P.pblk - 1));
+                        voff = slot * dma_s1 + dma_chunk;
+                        voff_v = slot * (uint32_t)P.sv1 + dma_chunk;
+                    } else {
+                        const uint32_t slot = (uint32_t)(key & (P.pblk - 1));
+                        sb += slot * dma_s1;
+                        sbv += slot * (uint32_t)P.sv1;
+                    }
+                    unsigned char* dst = ring + (wi & 1) * kWinBytes + u * TILE + wave * 1024;
+                    dma16_saddr(sb, voff, dst);
+                    if constexpr (B16) dma16_saddr(sbv, voff_v, dst + TILE / 2);
+                }
+            }
+        };
+        // Q as the B operand of S^T = K.Q^T: see prefill_attn.hip.  e4m3 caches: hi + lo parts, split by one wave per row-set
+        // and handed over through the LDS; bf16 caches: the four fragments, loaded by each wave.
+        auto load_query = [&](u32x4_t (&qf)[4], int tok, int head) {
+            const u32x4_t zero = {0u, 0u, 0u, 0u};
+            const bool ok = tok < qlen;
+            const __bf16* qrow = P.q + (int64_t)(q_begin + (ok ? tok : 0)) * P.q_stride + (int64_t)(kh * P.gqa + head) * kD;
+            qf[0] = ok ? load_16(qrow + 16 * lp) : zero;
+            qf[1] = ok ? load_16(qrow + 16 * lp + 8) : zero;
+            qf[2] = ok ? load_16(qrow + 64 + 16 * lp) : zero;
+            qf[3] = ok ? load_16(qrow + 64 + 16 * lp + 8) : zero;
+        };
+        v8i qhi[RS], qlo[RS];
+        float qkr[RS];
+        if (ntiles > 0) load_bids(0);
+        if constexpr (B16) {
+            u32x4_t qf[RS][4];
+#pragma unroll
+            for (int j = 0; j < RS; ++j) load_query(qf[j], token_of(j), head_of(grp * RS + j));
+#pragma unroll
+            for (int j = 0; j < RS; ++j) {
+                asm volatile("" : "+v"(qf[j][0]), "+v"(qf[j][1]), "+v"(qf[j][2]), "+v"(qf[j][3]));
+                qkr[j] = fmaxf(qk, kMinFactor16);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    qhi[j][d] = (int)(qf[j][0][d] ^ qflip);
+                    qhi[j][4 + d] = (int)(qf[j][1][d] ^ qflip);
+                    qlo[j][d] = (int)(qf[j][2][d] ^ qflip);
+                    qlo[j][4 + d] = (int)(qf[j][3][d] ^ qflip);
+                }
+            }
+            issue_window(0, 0, NT);
+            if (1 < nwin) load_bids(1);
+        } else {
+            constexpr int SETS = NG * RS, PER = (SETS + W - 1) / W;        // row-sets, and splits per wave at most
+            unsigned char* const exch = ring + kExch;
+            int ln = lane;                             // opaque: its addresses stay out of the key loop's registers
+            asm volatile("" : "+v"(ln));
+            u32x4_t qf[PER][4];
+#pragma unroll
+            for (int u = 0; u < PER; ++u) {
+                const int rset = wave + W * u;
+                load_query(qf[u], tok0 + 16 * block_of(rset) + lr, head_of(rset));
+            }
+#pragma unroll
+            for (int u = 0; u < PER; ++u)
+                asm volatile("" : "+v"(qf[u][0]), "+v"(qf[u][1]), "+v"(qf[u][2]), "+v"(qf[u][3]));
+            issue_window(0, 0, NT);
+            if (nwin > 0) load_scales(0);
+            if (1 < nwin) load_bids(1);
+#pragma unroll
+            for (int u = 0; u < PER; ++u) {
+                const int rset = wave + W * u;
+                if (rset < SETS) {
+                    v8i hi, lo;
+                    const float inv = q_fp8_split(qf[u], qflip, hi, lo);
+                    unsigned char* x = exch + rset * kSetBytes + 16 * ln;
+                    *reinterpret_cast<u32x4_t*>(x) = (u32x4_t){(uint32_t)hi[0], (uint32_t)hi[1], (uint32_t)hi[2], (uint32_t)hi[3]};
+                    *reinterpret_cast<u32x4_t*>(x + 1024) = (u32x4_t){(uint32_t)hi[4], (uint32_t)hi[5], (uint32_t)hi[6], (uint32_t)hi[7]};
+                    *reinterpret_cast<u32x4_t*>(x + 2048) = (u32x4_t){(uint32_t)lo[0], (uint32_t)lo[1], (uint32_t)lo[2], (uint32_t)lo[3]};
+                    *reinterpret_cast<u32x4_t*>(x + 3072) = (u32x4_t){(uint32_t)lo[4], (uint32_t)lo[5], (uint32_t)lo[6], (uint32_t)lo[7]};
+                    *reinterpret_cast<float*>(exch + rset * kSetBytes + 4096 + 4 * ln) = fmaxf(qk * inv, kMinFactor16);
+                }
+            }
+            lds_barrier();
+#pragma unroll
+            for (int j = 0; j < RS; ++j) {
+                const unsigned char* x = exch + (grp * RS + j) * kSetBytes + 16 * ln;
+                u32x4_t v[4];
+#pragma unroll
+                for (int d = 0; d < 4; ++d) v[d] = *reinterpret_cast<const u32x4_t*>(x + 1024 * d);
+                qhi[j] = (v8i){(int)v[0][0], (int)v[0][1], (int)v[0][2], (int)v[0][3],
+                               (int)v[1][0], (int)v[1][1], (int)v[1][2], (int)v[1][3]};
+                qlo[j] = (v8i){(int)v[2][0], (int)v[2][1], (int)v[2][2], (int)v[2][3],
+                               (int)v[3][0], (int)v[3][1], (int)v[3][2], (int)v[3][3]};
+                qkr[j] = *reinterpret_cast<const float*>(exch + (grp * RS + j) * kSetBytes + 4096 + 4 * ln);
+            }
+        }
+
+        float m_run[RS], l_run[RS];
+        f32x4_t o[RS][8];
+#pragma unroll
+        for (int j = 0; j < RS; ++j) {
+            m_run[j] = kMaxFloor;
+            l_run[j] = 0.f;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) o[j][n] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+        }
+        [[maybe_unused]] float e_run[RS] = {};
+
+        for (int i = 0; i < nwin; ++i) {
+            // Everything this wave has in flight: window i's copies and scales, the block ids of window i + 1.  The
+            // barrier then publishes window i and frees window i - 1's slot.
+            wait_vmcnt<0>();
+            if constexpr (SC) {
+                if ((wave == 0 || wave == 2) && lane < NT) lds_scales[i & 1][lane][wave >> 1] = (uint16_t)sc_next;
+            }
+            lds_barrier();
+            const bool more = i + 1 < nwin;
+
+#pragma unroll
+            for (int v = 0; v < TPW; ++v) {
+                // The next window's copies go out in TPW parts, one before each tile.
+                if (more) {
+                    issue_window(i + 1, v * NT / TPW, (v + 1) * NT / TPW);
+                    if (v == 0) load_scales(i + 1);
+                }
+                const int tw = res * TPW + v;                    // tile within the window
+                const int t = i * NT + tw;
+                const int k0 = kBN * tile_at(t);
+                if (t >= ntiles || (MB && (k0 > my_hi || (k0 + kBN <= my_low && k0 >= sinks)))) continue;
+                const unsigned char* buf = ring + (i & 1) * kWinBytes + tw * TILE;
+                // Some row does not see some key: past the first query, or below the last one's window and no sink.
+                const bool masked = k0 + kBN - 1 > qfirst || (k0 <= qlast - window && k0 + kBN > sinks);
+                f32x4_t sc[RS][2];
+                bool poisoned = false;
+                if constexpr (B16) {
+                    if (masked) {
+                        int ln = lane;                 // opaque, as above
+                        asm volatile("" : "+v"(ln));
+                        uint32_t bad = 0;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            const u32x4_t w = *reinterpret_cast<const u32x4_t*>(buf + TILE / 2 + 1024 * c + 16 * ln);
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) bad |= non_finite<true>(w[d]);
+                        }
+                        poisoned = __any(bad != 0);
+                    }
+#pragma unroll
+                    for (int kg = 0; kg < 2; ++kg) {
+                        const int row = 16 * kg + lr;
+                        u32x4_t kf[4];
+#pragma unroll
+                        for (int f = 0; f < 4; ++f)
+                            kf[f] = *reinterpret_cast<const u32x4_t*>(buf + b16_slot(row, 8 * (f >> 1) + 2 * lp + (f & 1)));
+#pragma unroll
+                        for (int j = 0; j < RS; ++j) {
+                            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int f = 0; f < 4; ++f) {
+                                const v8i& qq = f < 2 ? qhi[j] : qlo[j];
+                                const int h = 4 * (f & 1);
+                                const u32x4_t qv = {(uint32_t)qq[h], (uint32_t)qq[h + 1], (uint32_t)qq[h + 2],
+                                                    (uint32_t)qq[h + 3]};
+                                acc = mfma16x16x32_bf16(as_bf16x8(kf[f]), as_bf16x8(qv), acc);
+                            }
+                            sc[j][kg] = acc;
+                        }
+                    }
+                }
+                [[maybe_unused]] u32x4_t vf[HALVES ? 4 : 8];
+                [[maybe_unused]] uint32_t vhalf[8];
+                [[maybe_unused]] float ev[2];
+                // fp16 V^T fragments 4 w .. 4 w + 3 (d = 8c + 4w ..) from word w of the eight rows
+                auto widen_words = [&](const uint32_t (&r)[8], int w) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t x = __builtin_amdgcn_perm(r[2 * k + 1], r[2 * k], 0x05010400u);   // a0 b0 a1 b1
+                        const uint32_t y = __builtin_amdgcn_perm(r[2 * k + 1], r[2 * k], 0x07030602u);   // a2 b2 a3 b3
+                        const int at = HALVES ? 0 : 4 * w;
+                        vf[at + 0][k] = f16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x, 1.0f, false));
+                        vf[at + 1][k] = f16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x, 1.0f, true));
+                        vf[at + 2][k] = f16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)y, 1.0f, false));
+                        vf[at + 3][k] = f16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)y, 1.0f, true));
+                    }
+                };
+                auto widen = [&](const u32x2_t (&vr)[8], int w) {
+                    const uint32_t r[8] = {vr[0][w], vr[1][w], vr[2][w], vr[3][w], vr[4][w], vr[5][w], vr[6][w], vr[7][w]};
+                    widen_words(r, w);
+                };
+                if constexpr (!B16) {
+                    v8i kf[2];
+#pragma unroll
+                    for (int kg = 0; kg < 2; ++kg) {
+                        const int row = 16 * kg + lr;
+                        const unsigned char* kb = buf + (row >> 3) * 1024;
+                        const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(kb + 16 * k_slot(row & 7, lp));
+                        const u32x4_t hi = *reinterpret_cast<const u32x4_t*>(kb + 16 * k_slot(row & 7, 4 + lp));
+                        kf[kg] = (v8i){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3],
+                                       (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+                    }
+                    uint32_t scales = 127 | 127 << 16;
+                    if constexpr (SC) {
+                        scales = *reinterpret_cast<const uint32_t*>(lds_scales[i & 1][tw]);
+                        ev[0] = uniform((float)((int)((scales >> 8) & 255u) - 127));
+                        ev[1] = uniform((float)((int)(scales >> 24) - 127));
+                    }
+                    // V^T raw rows (lane (c, p) transposes d = 8c .. 8c+7) and their widening go ahead of S^T = K.Q^T
+                    u32x2_t vr[8];
+#pragma unroll
+                    for (int jj = 0; jj < 8; ++jj) {
+                        const int row = (jj < 4 ? 0 : 16) + 4 * lp + (jj & 3);
+                        const unsigned char* vb = buf + 4096 + (row >> 3) * 1024;
+                        vr[jj] = *reinterpret_cast<const u32x2_t*>(vb + 16 * v_slot(row & 7, lr >> 1) + 8 * (lr & 1));
+                    }
+                    if (masked) {
+                        uint32_t bad = 0;
+#pragma unroll
+                        for (int jj = 0; jj < 8; ++jj) bad |= non_finite<false>(vr[jj][0]) | non_finite<false>(vr[jj][1]);
+                        poisoned = __any(bad != 0);
+                        if (poisoned) {
+#pragma unroll
+                            for (int jj = 0; jj < 8; ++jj) {
+                                vr[jj][0] = finite_only<false>(vr[jj][0]);
+                                vr[jj][1] = finite_only<false>(vr[jj][1]);
+                            }
+                        }
+                    }
+                    if constexpr (!HALVES) {
+                        widen(vr, 0);
+                        widen(vr, 1);
+                    }
+#pragma unroll
+                    for (int j = 0; j < RS; ++j) {
+                        const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
+                        f32x4_t acc = score_mfma<0, false>(kf[0], qhi[j], zero, scales);
+                        sc[j][0] = score_mfma<0, true>(kf[0], qlo[j], acc, scales);
+                        acc = score_mfma<1, false>(kf[1], qhi[j], zero, scales);
+                        sc[j][1] = score_mfma<1, true>(kf[1], qlo[j], acc, scales);
+                    }
+                    if constexpr (HALVES) {
+#pragma unroll
+                        for (int jj = 0; jj < 8; ++jj) {
+                            asm volatile("" : "+v"(vr[jj][0]), "+v"(vr[jj][1]));
+                            vhalf[jj] = vr[jj][1];
+                        }
+                        widen(vr, 0);
+                    } else {
+                        // Interleave: one MFMA, then up to four VALU (the V widening, 48 instructions).
+#pragma unroll
+                        for (int g = 0; g < 4 * RS; ++g) {
+                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                        }
+                    }
+                }
+                if (masked) {
+                    int lm = lane;                     // opaque, as above
+                    asm volatile("" : "+v"(lm));
+#pragma unroll
+                    for (int j = 0; j < RS; ++j) {
+                        const int qpos = q0 + tok0 + 16 * block_of(grp * RS + j) + (lm & 15);
+#pragma unroll
+                        for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int key = k0 + 16 * kg + 4 * (lm >> 4) + e;
+                                if (key > qpos || (key <= qpos - window && key >= sinks)) sc[j][kg][e] = neg_inf();
+                            }
+                    }
+                }
+                // Weights of row-set j in the type of P.V (the P^T operand), their sum added to l.  The product is rounded
+                // like the row max, so the largest weight is at most 2^kRescaleSlack at any score.
+                auto row_probs = [&](int j) -> u32x4_t {
+#pragma clang fp contract(off)
+                    const float nm = -m_run[j];
+                    float p[2][4];
+#pragma unroll
+                    for (int kg = 0; kg < 2; ++kg)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[kg][e] = __builtin_amdgcn_exp2f(sc[j][kg][e] * qkr[j] + nm);
+                    [[maybe_unused]] float f[2];
+                    if constexpr (SC) {                // a group whose keys are all masked may lie far above the row's unit
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) f[g] = __builtin_amdgcn_exp2f(fminf(ev[g] - e_run[j], 120.f));
+                    }
+                    u32x4_t pb;
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        float& a = p[d >> 1][2 * (d & 1)];
+                        float& b = p[d >> 1][2 * (d & 1) + 1];
+                        if constexpr (SC) pb[d] = pack_f16x2(a * f[d >> 1], b * f[d >> 1]);
+                        else pb[d] = B16 ? pack_bf16x2(a, b) : pack_f16x2(a, b);
+                        if (B16) {
+                            a = __uint_as_float(pb[d] << 16);
+                            b = __uint_as_float(pb[d] & 0xFFFF0000u);
+                        }
+                    }
+                    l_run[j] += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+                    return pb;
+                };
+                if constexpr (!B16) {
+                    if constexpr (SC) rescale_rows_scaled<RS>(sc, m_run, l_run, o, qkr, e_run, ev);
+                    else rescale_rows<RS>(sc, m_run, l_run, o, qkr);
+                    if constexpr (HALVES) {
+                        u32x4_t pb[RS];
+#pragma unroll
+                        for (int j = 0; j < RS; ++j) {
+                            pb[j] = row_probs(j);
+#pragma unroll
+                            for (int n = 0; n < 4; ++n) o[j][n] = mfma16x16x32_f16(vf[n], pb[j], o[j][n]);
+                        }
+                        widen_words(vhalf, 1);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+#pragma unroll
+                            for (int j = 0; j < RS; ++j) o[j][4 + n] = mfma16x16x32_f16(vf[n], pb[j], o[j][4 + n]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < RS; ++j) {
+                            const u32x4_t pb = row_probs(j);
+#pragma unroll
+                            for (int n = 0; n < 8; ++n) o[j][n] = mfma16x16x32_f16(vf[n], pb, o[j][n]);
+                        }
+                    }
+                    // Interleave: the first row-set's exponentials alone, then each P.V MFMA with about three
+                    // VALU instructions of the next row-set's softmax.
+                    if constexpr (!HALVES) {
+                        __builtin_amdgcn_sched_group_barrier(0x002, 28, 0);
+#pragma unroll
+                        for (int g = 0; g < 8 * (RS - 1); ++g) {
+                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+                        }
+                    }
+                } else {
+                    // Half of a V row's 16 bytes at a time: half h is d = 8c + 4h .. + 3.
+                    u32x2_t vr[8];
+                    auto read_half = [&](int h) {
+#pragma unroll
+                        for (int jj = 0; jj < 8; ++jj) {
+                            const int row = (jj < 4 ? 0 : 16) + 4 * lp + (jj & 3);
+                            vr[jj] = *reinterpret_cast<const u32x2_t*>(buf + TILE / 2 + b16_slot(row, lr) + 8 * h);
+                        }
+                        if (poisoned) {
+#pragma unroll
+                            for (int jj = 0; jj < 8; ++jj) {
+                                vr[jj][0] = finite_only<true>(vr[jj][0]);
+                                vr[jj][1] = finite_only<true>(vr[jj][1]);
+                            }
+                        }
+                    };
+                    read_half(0);
+                    rescale_rows<RS>(sc, m_run, l_run, o, qkr);
+                    u32x4_t pb[RS];
+#pragma unroll
+                    for (int j = 0; j < RS; ++j) pb[j] = row_probs(j);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        u32x4_t va[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+#pragma unroll
+                            for (int w = 0; w < 2; ++w) {
+                                va[2 * w][k] = __builtin_amdgcn_perm(vr[2 * k + 1][w], vr[2 * k][w], 0x05040100u);
+                                va[2 * w + 1][k] = __builtin_amdgcn_perm(vr[2 * k + 1][w], vr[2 * k][w], 0x07060302u);
+                            }
+                        if (h == 0) read_half(1);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+#pragma unroll
+                            for (int j = 0; j < RS; ++j)
+                                o[j][4 * h + n] = mfma16x16x32_bf16(as_bf16x8(va[n]), as_bf16x8(pb[j]), o[j][4 * h + n]);
+                    }
+                }
+                if (poisoned) {
+                    // The non-finite V elements of the tile, key by key, to the rows that see them: lane (q, p) holds
+                    // d = 32 p + 8 i + n.
+                    int ln = lane;                     // opaque: nothing of this stays in registers through the key loop
+                    asm volatile("" : "+v"(ln));
+                    const int part = ln >> 4;
+                    for (int row = 0; row < kBN; ++row) {
+                        const int key = k0 + row;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int d = 0; d < (B16 ? 4 : 2); ++d) {
+                                const unsigned char* src = B16 ? buf + TILE / 2 + b16_slot(row, 4 * part + e)
+                                    : buf + TILE / 2 + (row >> 3) * 1024 + 16 * v_slot(row & 7, 2 * part + (e >> 1)) + 8 * (e & 1);
+                                const uint32_t w = reinterpret_cast<const uint32_t*>(src)[d];
+                                if (!__any(non_finite<B16>(w) != 0)) continue;
+#pragma unroll
+                                for (int j = 0; j < RS; ++j) {
+                                    const int qpos = q0 + tok0 + 16 * block_of(grp * RS + j) + (ln & 15);
+                                    const bool sees = key <= qpos && (key > qpos - window || key < sinks);
+                                    constexpr int per = B16 ? 2 : 4;               // elements of a word
+#pragma unroll
+                                    for (int h = 0; h < per; ++h) {
+                                        float x;
+                                        if constexpr (B16) {
+                                            const uint32_t bits = h ? w & 0xFFFF0000u : w << 16;
+                                            x = (bits & 0x7F800000u) == 0x7F800000u ? __uint_as_float(bits) : 0.f;
+                                        } else {
+                                            x = ((w >> (8 * h)) & 0x7Fu) == 0x7Fu ? __builtin_nanf("") : 0.f;
+                                        }
+                                        o[j][per * d + h][e] += sees ? x : 0.f;
+                                    }
+                                }
+                            }
+                    }
+                }
+            }
+            // Block ids for the next window's copies, after this iteration's LDS reads.
+            if (i + 2 < nwin) load_bids(i + 2);
+        }
+
+        int ln = lane;                                 // opaque, as above
+        asm volatile("" : "+v"(ln));
+        const int er = ln & 15, ep = ln >> 4;
+        // ---- merge the NR partial states of each head group, then normalise and store ----------
+        if constexpr (NR > 1) {
+            // m_run is the same in the four lane groups of a query row: lanes 0..15 publish it.
+            if (ep == 0) {
+#pragma unroll
+                for (int j = 0; j < RS; ++j) stage_m[((grp * NR + res) * RS + j) * 16 + er] = m_run[j];
+            }
+            lds_barrier();
+#pragma unroll
+            for (int j = 0; j < RS; ++j) {
+                float mg = kMaxFloor;
+#pragma unroll
+                for (int r = 0; r < NR; ++r) mg = fmaxf(mg, stage_m[((grp * NR + r) * RS + j) * 16 + er]);
+                const float f = __builtin_amdgcn_exp2f(m_run[j] - mg);
+                const float fo = SC ? __builtin_amdgcn_exp2f((m_run[j] - mg) + e_run[j]) : f;
+                l_run[j] *= f;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) o[j][n] *= fo;
+            }
+            // Row-set j is summed and written by residue j % NR, in the order of the residues behind it.
+#pragma unroll
+            for (int j = 0; j < RS; ++j) {
+                if (res == j % NR) continue;
+                const int slot = (res - j % NR + NR) % NR - 1;
+                float* s = stage + (((grp * RS + j) * (NR - 1)) + slot) * kStageFloats;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) *reinterpret_cast<f32x4_t*>(s + (n * 64 + ln) * 4) = o[j][n];
+                s[8 * 64 * 4 + ln] = l_run[j];
+            }
+            lds_barrier();
+#pragma unroll
+            for (int j = 0; j < RS; ++j) {
+                if (res != j % NR) continue;
+#pragma unroll
+                for (int r = 0; r < NR - 1; ++r) {
+                    const float* s = stage + ((grp * RS + j) * (NR - 1) + r) * kStageFloats;
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) o[j][n] += *reinterpret_cast<const f32x4_t*>(s + (n * 64 + ln) * 4);
+                    l_run[j] += s[8 * 64 * 4 + ln];
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < RS; ++j) {
+            if (res != j % NR) continue;
+            const float l = sum_xor16_32(l_run[j]);
+            const int tok = tok0 + 16 * block_of(grp * RS + j) + er;
+            if (tok >= qlen || grp * RS + j >= nbt * P.gqa) continue;
+            // a row that sees no key has l = 0 and is written as zeros; NaN in l reaches the output
+            float f = l == 0.f ? 0.f : vs / l;
+            if constexpr (SC && NR == 1) f *= __builtin_amdgcn_exp2f(e_run[j]);
+            __bf16* orow = P.out + (int64_t)(q_begin + tok) * P.o_stride +
+                           (int64_t)(kh * P.gqa + head_of(grp * RS + j)) * kD + 32 * ep;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                u32x4_t w;
+                w[0] = pack_bf16x2(o[j][0][e] * f, o[j][1][e] * f);
+                w[1] = pack_bf16x2(o[j][2][e] * f, o[j][3][e] * f);
+                w[2] = pack_bf16x2(o[j][4][e] * f, o[j][5][e] * f);
+                w[3] = pack_bf16x2(o[j][6][e] * f, o[j][7][e] * f);
+                *reinterpret_cast<u32x4_t*>(orow + 8 * e) = w;
+            }
+        }
+        // The next block's copies overwrite the ring, which holds the stage: every wave must be
+        // done with its final stage reads above.
+        if (ph + 1 < nphase) lds_barrier();
+    }
+}
+
+template <bool SC>
+void launch_e4m3(const VisibleParams& P, dim3 grid, dim3 block, hipStream_t stream)
+{
+    const int g = P.gqa;
+    if (g <= 2) launch_kernel(prefill_visible_kernel<2, 2, 2, false, true, SC>, grid, block, 0, stream, P);
+    else if (g <= 4) launch_kernel(prefill_visible_kernel<2, 2, 2, false, false, SC>, grid, block, 0, stream, P);
+    else if (g <= 6) launch_kernel(prefill_visible_kernel<3, 2, 2, false, false, SC>, grid, block, 0, stream, P);
+    else if (g <= 8) launch_kernel(prefill_visible_kernel<2, 4, 2, false, false, SC>, grid, block, 0, stream, P);
+    else if (g <= 12) launch_kernel(prefill_visible_kernel<3, 4, 2, false, false, SC>, grid, block, 0, stream, P);
+    else launch_kernel(prefill_visible_kernel<2, 8, 2, false, false, SC>, grid, block, 0, stream, P);
+}
+
+// Whole causal contexts: pairs of blocks (r, n - 1 - r) where single ones overflow a round of workgroups, as in
+// prefill_attn.hip.  With a window the blocks cost alike, and pairs would only halve the workgroups to
+// choose from.
+int launch_visible(const VisibleParams& P0, bool b16, int num_seqs, int max_query_len, hipStream_t stream)
+{
+    VisibleParams P = P0;
+    const int g = P.gqa;
+    P.nb = split_blocks(g);
+    const int n = (max_query_len + 16 * P.nb - 1) / (16 * P.nb);
+    P.xcd_map = (P.hkv <= 8 && 8 % P.hkv == 0) ? 1 : 0;
+    P.paired = P.window == 0 && !split_single_blocks_fit(n, P.hkv, num_seqs);
+    const int per = split_xcd_per(P.hkv), ranks = P.paired ? (n + 1) / 2 : n;
+    P.ntb_grid = (ranks + per - 1) / per * per;
+    const dim3 grid((unsigned)(P.ntb_grid * P.hkv), 1u, (unsigned)num_seqs), block(64 * kSplitWaves);
+    begin_launch();
+    if (b16) {
+        if (g <= 2) launch_kernel(prefill_visible_kernel<2, 2, 1, true, true, false>, grid, block, 0, stream, P);
+        else if (g <= 4) launch_kernel(prefill_visible_kernel<2, 2, 1, true, false, false>, grid, block, 0, stream, P);
+        else if (g <= 6) launch_kernel(prefill_visible_kernel<3, 2, 1, true, false, false>, grid, block, 0, stream, P);
+        else if (g <= 8) launch_kernel(prefill_visible_kernel<2, 4, 2, true, false, false>, grid, block, 0, stream, P);
+        else launch_kernel(prefill_visible_kernel<2, 8, 4, true, false, false>, grid, block, 0, stream, P);
+    } else if (P.kv_scales) {
+        launch_e4m3<true>(P, grid, block, stream);
+    } else {
+        launch_e4m3<false>(P, grid, block, stream);
+    }
+    return finish_launch();
+}
+
+enum CacheKind { kE4m3 = 0, kBf16 = 1, kBlk = 2 };
+
+template <int KIND>
+int prefill_visible(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache, int64_t sk0, int64_t sk1,
+                    int64_t sk2, int64_t sv0, int64_t sv1, int64_t sv2, void* out, int64_t out_row_stride,
+                    const int32_t* cu_seqlens_q, const int32_t* seq_lens, const int32_t* block_table, int64_t bt_stride,
+                    const float* k_scale, const float* v_scale, const void* kv_scales, float sm_scale, int num_seqs,
+                    int num_q_heads, int num_kv_heads, int head_size, int block_size, int window, int sinks,
+                    int max_query_len, void* stream)
+{
+    if (!cu_seqlens_q || !seq_lens || num_seqs < 1 || max_query_len < 0 || window < 0 || sinks < 0) return FP8KV_ERR_ARG;
+    if (KIND == kBlk && !kv_scales) return FP8KV_ERR_ARG;
+    if (num_seqs > 65535) return FP8KV_ERR_SHAPE;
+    const int64_t elem = KIND == kBf16 ? 2 : 1;
+    sk0 *= elem; sk1 *= elem; sk2 *= elem;
+    sv0 *= elem; sv1 *= elem; sv2 *= elem;
+    const float* any = reinterpret_cast<const float*>(q);           // scales that only the kE4m3 kernels read
+    const int st = check_common(q, k_cache, v_cache, out, q_row_stride, sk0, sk1, sk2, sv0, sv1, sv2, block_table, bt_stride,
+                                KIND == kE4m3 ? k_scale : any, KIND == kE4m3 ? v_scale : any, num_q_heads, num_kv_heads,
+                                head_size, block_size, out_row_stride);
+    if (st != FP8KV_OK) return st;
+    if (KIND == kBf16 && (!aligned(v_cache, 16) || ((sv0 | sv1 | sv2) & 15))) return FP8KV_ERR_ALIGN;
+    if (KIND == kBlk && !aligned(kv_scales, 2)) return FP8KV_ERR_ALIGN;
+    if (max_query_len == 0) return FP8KV_OK;
+    VisibleParams P;
+    static_cast<Params&>(P) = make_params(q, q_row_stride, k_cache, v_cache, sk0, sk1, sk2, sv0, sv1, sv2, out, out_row_stride,
+                                          block_table, bt_stride, k_scale, v_scale, sm_scale, num_q_heads, num_kv_heads,
+                                          block_size);
+    P.cu_q = cu_seqlens_q;
+    P.seq_lens = seq_lens;
+    P.kv_scales = static_cast<const uint16_t*>(kv_scales);
+    P.window = window;
+    P.sinks = sinks;
+    return launch_visible(P, KIND == kBf16, num_seqs, max_query_len, reinterpret_cast<hipStream_t>(stream));
+}
+
+}  // namespace prefill_detail
+}  // namespace fp8kv
+
+using namespace fp8kv::prefill_detail;
+
+extern "C" int fp8kv_prefill_attn_window(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                         int64_t sk0, int64_t sk1, int64_t sk2, int64_t sv0, int64_t sv1, int64_t sv2,
+                                         void* out, int64_t out_row_stride, const int32_t* cu_seqlens_q,
+                                         const int32_t* seq_lens, const int32_t* block_table, int64_t bt_stride,
+                                         const float* k_scale, const float* v_scale, float sm_scale, int num_seqs,
+                                         int num_q_heads, int num_kv_heads, int head_size, int block_size, int window,
+                                         int sinks, int max_query_len, void* stream)
+{
+    return prefill_visible<kE4m3>(q, q_row_stride, k_cache, v_cache, sk0, sk1, sk2, sv0, sv1, sv2, out, out_row_stride,
+                                  cu_seqlens_q, seq_lens, block_table, bt_stride, k_scale, v_scale, nullptr, sm_scale, num_seqs,
+                                  num_q_heads, num_kv_heads, head_size, block_size, window, sinks, max_query_len, stream);
+}
+
+extern "C" int fp8kv_prefill_attn_window_bf16(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                              int64_t sk0, int64_t sk1, int64_t sk2, int64_t sv0, int64_t sv1, int64_t sv2,
+                                              void* out, int64_t out_row_stride, const int32_t* cu_seqlens_q,
+                                              const int32_t* seq_lens, const int32_t* block_table, int64_t bt_stride,
+                                              float sm_scale, int num_seqs, int num_q_heads, int num_kv_heads, int head_size,
+                                              int block_size, int window, int sinks, int max_query_len, void* stream)
+{
+    return prefill_visible<kBf16>(q, q_row_stride, k_cache, v_cache, sk0, sk1, sk2, sv0, sv1, sv2, out, out_row_stride,
+                                  cu_seqlens_q, seq_lens, block_table, bt_stride, nullptr, nullptr, nullptr, sm_scale, num_seqs,
+                                  num_q_heads, num_kv_heads, head_size, block_size, window, sinks, max_query_len, stream);
+}
+
+extern "C" int fp8kv_prefill_attn_blk(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                      int64_t sk0, int64_t sk1, int64_t sk2, int64_t sv0, int64_t sv1, int64_t sv2,
+                                      void* out, int64_t out_row_stride, const int32_t* cu_seqlens_q, const int32_t* seq_lens,
+                                      const int32_t* block_table, int64_t bt_stride, const void* kv_scales, float sm_scale,
+                                      int num_seqs, int num_q_heads, int num_kv_heads, int head_size, int block_size,
+                                      int window, int sinks, int max_query_len, void* stream)
+{
+    return prefill_visible<kBlk>(q, q_row_stride, k_cache, v_cache, sk0, sk1, sk2, sv0, sv1, sv2, out, out_row_stride,
+                                 cu_seqlens_q, seq_lens, block_table, bt_stride, nullptr, nullptr, kv_scales, sm_scale, num_seqs,
+                                 num_q_heads, num_kv_heads, head_size, block_size, window, sinks, max_query_len, stream);
+}

@@ -17,6 +17,8 @@ _c_i64 = ctypes.c_int64
 _c_f = ctypes.c_float
 _c_sz = ctypes.c_size_t
 
+# The leading arguments of the attention entry points over sequences, up to the block table's stride.
+_DECODE = [_c_vp, _c_i64, _c_vp, _c_vp] + [_c_i64] * 6 + [_c_vp, _c_i64] + [_c_vp] * 3 + [_c_i64]
 # The leading arguments of the rope_append entry points, up to `interleaved`.
 _ROPE_APPEND = [_c_vp, _c_i64] * 4 + [_c_vp] * 2 + [_c_i64] * 6 + [_c_vp, _c_vp, _c_i64, _c_i, _c_i64, _c_i, _c_i]
 
@@ -62,6 +64,14 @@ SIGNATURES: dict[str, tuple] = {
     # fp8 KV-cache write (csrc/cache_write.hip)
     "fp8kv_cache_write": (_c_i, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp] + [_c_i64] * 6
                           + [_c_vp] * 3 + [_c_i] * 4 + [_c_vp]),
+    # attention over the visible keys of a window, and over block-scaled caches (csrc/decode_attn.hip,
+    # csrc/prefill_visible.hip)
+    "fp8kv_decode_attn_window": (_c_i, _DECODE + [_c_vp] * 2 + [_c_f] + [_c_i] * 6 + [_c_vp, _c_sz] + [_c_i] * 3 + [_c_vp]),
+    "fp8kv_decode_attn_window_bf16": (_c_i, _DECODE + [_c_f] + [_c_i] * 6 + [_c_vp, _c_sz] + [_c_i] * 3 + [_c_vp]),
+    "fp8kv_decode_attn_blk": (_c_i, _DECODE + [_c_vp, _c_f] + [_c_i] * 6 + [_c_vp, _c_sz] + [_c_i] * 3 + [_c_vp]),
+    "fp8kv_prefill_attn_window": (_c_i, _DECODE + [_c_vp] * 2 + [_c_f] + [_c_i] * 8 + [_c_vp]),
+    "fp8kv_prefill_attn_window_bf16": (_c_i, _DECODE + [_c_f] + [_c_i] * 8 + [_c_vp]),
+    "fp8kv_prefill_attn_blk": (_c_i, _DECODE + [_c_vp, _c_f] + [_c_i] * 8 + [_c_vp]),
     # position rotation and cache append in one pass (csrc/rope_append.hip)
     "fp8kv_rope_append": (_c_i, _ROPE_APPEND + [_c_vp] * 3 + [_c_i] * 5 + [_c_i64, _c_vp]),
     "fp8kv_rope_append_bf16": (_c_i, _ROPE_APPEND + [_c_vp] + [_c_i] * 5 + [_c_i64, _c_vp]),

@@ -20,7 +20,7 @@ INCLUDE = os.path.join(REPO_ROOT, "include")
 LIB_NAME = "libfp8kv_amd.so"
 LIB_PATH = os.path.join(PKG_ROOT, LIB_NAME)
 
-SOURCES = ["h4mv.hip", "h4mv_repack.hip", "decode_attn.hip", "prefill_attn.hip", "prefill_bf16kv.hip",
+SOURCES = ["h4mv.hip", "h4mv_repack.hip", "decode_attn.hip", "prefill_attn.hip", "prefill_bf16kv.hip", "prefill_visible.hip",
            "cache_write.hip", "rope_append.hip", "epilogues.hip", "w4a8_gemm.hip", "w4a8_slice.hip", "lm_head.hip"]
 # The benchmark's read-only reference launch (fp8kv_stream_read) is a measurement aid, not part of
 # the path: it is built into a library of its own that only bench.py loads.

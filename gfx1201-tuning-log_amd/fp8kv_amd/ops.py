@@ -510,6 +510,133 @@ def rope_append_blk(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tens
     return q_out
 
 
+# ------------------------------------------------------------------------------ attention over visible keys
+
+def _visible_checks(q, k_cache, v_cache, out, starts, seq_lens, block_table, window, sinks):
+    """Checks what the calls below share; (leading arguments, trailing geometry) of the C calls."""
+    T, HQ, D = q.shape if q.dim() == 3 else (0, 0, 0)
+    for t, n in ((q, "q"), (out, "out")):
+        if not (t.dtype == torch.bfloat16 and t.dim() == 3 and t.is_cuda and t.stride(2) == 1 and
+                (t.stride(1) == D or HQ == 1) and t.shape[1:] == q.shape[1:]):
+            raise ValueError(f"{n} must be bf16 [T, HQ, D] with contiguous heads")
+    dev = q.device
+    if not (k_cache.shape == v_cache.shape and k_cache.shape[3] == D):
+        raise ValueError("caches must be [NB, PBLK, HKV, D] of q's head size")
+    for t, n in ((starts, "query_start_loc"), (seq_lens, "seq_lens"), (block_table, "block_table")):
+        if not (t.dtype == torch.int32 and t.device == dev and (t.stride(-1) == 1 or t.shape[-1] == 1)):
+            raise ValueError(f"{n} must be an int32 tensor on q's device, contiguous along its last axis")
+    NS = block_table.shape[0]
+    if not (block_table.dim() == 2 and starts.shape == (NS + 1,) and seq_lens.shape == (NS,)):
+        raise ValueError("block_table must be [NS, max_blocks], query_start_loc [NS + 1], seq_lens [NS]")
+    if not (out.device == k_cache.device == v_cache.device == dev):
+        raise ValueError("tensors on different devices")
+    if not (window >= 0 and sinks >= 0):
+        raise ValueError("window and sinks must not be negative")
+    lead = (q.data_ptr(), _row_stride(q), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+            v_cache.stride(0), v_cache.stride(1), v_cache.stride(2),
+            out.data_ptr(), _row_stride(out), starts.data_ptr(), seq_lens.data_ptr(),
+            block_table.data_ptr(), block_table.stride(0))
+    return lead, (NS, HQ, k_cache.shape[2], D, k_cache.shape[1])
+
+
+def _decode_visible(name, q, out, lead, scales, sm_scale, geometry, seq_lens, window, sinks, num_splits, max_seq_len,
+                    scratch, bf16_kv):
+    NS, HQ, HKV, D, _ = geometry
+    if NS == 0:
+        return out
+    if num_splits is None:
+        if max_seq_len is None and window == 0:
+            max_seq_len = int(seq_lens.max().item())
+        visible = window + sinks if max_seq_len is None else max_seq_len
+        if window > 0:
+            visible = min(visible, window + sinks)
+        num_splits = decode_num_splits(NS, HKV, min(int(visible), 1 << 30), bf16_kv)
+    need = decode_scratch_bytes(NS, HQ, HKV, num_splits, D)
+    if scratch is None:
+        scratch = _call_scratch(need, q.device)
+    elif need > 0:
+        if not (scratch.is_cuda and scratch.numel() * scratch.element_size() >= need):
+            raise ValueError(f"scratch needs {need} bytes")
+    sbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
+    _launch(name, q, *lead, *scales, float(sm_scale), *geometry, int(num_splits), _ptr(scratch), sbytes, int(window),
+            int(sinks), int(max_seq_len or 0))
+    return out
+
+
+def _prefill_visible(name, q, out, lead, scales, sm_scale, geometry, starts, window, sinks, max_query_len):
+    if max_query_len is None:
+        max_query_len = int((starts[1:] - starts[:-1]).max().item()) if geometry[0] else 0
+    if q.shape[0] > 0 and geometry[0] > 0:
+        _launch(name, q, *lead, *scales, float(sm_scale), *geometry, int(window), int(sinks), int(max_query_len))
+    return out
+
+
+def _per_tensor_scales(k_cache, v_cache, k_scale, v_scale, dev):
+    """(suffix of the entry point, its scale arguments, tensors that must live until the launch)."""
+    if _kv_caches_bf16(k_cache, v_cache):
+        return "_bf16", (), ()
+    ks, vs = _scale_tensor(k_scale, dev), _scale_tensor(v_scale, dev)
+    return "", (ks.data_ptr(), vs.data_ptr()), (ks, vs)
+
+
+def decode_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor,
+                            query_start_loc: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor,
+                            k_scale, v_scale, sm_scale: float, window: int, sinks: int = 0,
+                            num_splits: int | None = None, max_seq_len: int | None = None,
+                            scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """``decode_attention`` where the query of sequence s, at position p = seq_lens[s] - 1, sees only the keys
+    t > p - window and the first ``sinks`` ones (window 0: all).  Caches e4m3 with per-tensor scales, or bf16.
+
+    Only the visible keys are read; block-table entries of blocks that hold none may be anything.  A window bounds
+    the work, so ``max_seq_len`` is needed only without one (and then read from ``seq_lens``, which synchronises)."""
+    suffix, scales, keep = _per_tensor_scales(k_cache, v_cache, k_scale, v_scale, q.device)
+    lead, geometry = _visible_checks(q, k_cache, v_cache, out, query_start_loc, seq_lens, block_table, window, sinks)
+    return _decode_visible("fp8kv_decode_attn_window" + suffix, q, out, lead, scales, sm_scale, geometry, seq_lens, window,
+                           sinks, num_splits, max_seq_len, scratch, suffix == "_bf16")
+
+
+def prefill_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor,
+                             cu_seqlens_q: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor,
+                             k_scale, v_scale, sm_scale: float, window: int, sinks: int = 0,
+                             max_query_len: int | None = None) -> torch.Tensor:
+    """``prefill_attention_varlen`` where the query at position p sees the keys t <= p with t > p - window
+    or t < sinks (window 0: all t <= p).  Caches e4m3 with per-tensor scales, or bf16."""
+    suffix, scales, keep = _per_tensor_scales(k_cache, v_cache, k_scale, v_scale, q.device)
+    lead, geometry = _visible_checks(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, window, sinks)
+    return _prefill_visible("fp8kv_prefill_attn_window" + suffix, q, out, lead, scales, sm_scale, geometry, cu_seqlens_q,
+                            window, sinks, max_query_len)
+
+
+def decode_attention_blk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor,
+                         query_start_loc: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor,
+                         kv_scales: torch.Tensor, sm_scale: float, window: int = 0, sinks: int = 0,
+                         num_splits: int | None = None, max_seq_len: int | None = None,
+                         scratch: torch.Tensor | None = None) -> torch.Tensor:
+    """``decode_attention`` over the block-scaled e4m3 cache that ``rope_append_blk`` writes (``kv_scales`` uint8
+    [NB, PBLK / 16, HKV, 2]), with ``window`` and ``sinks`` as in ``decode_attention_window``."""
+    _fp8_cache_check(k_cache, "k_cache")
+    _fp8_cache_check(v_cache, "v_cache")
+    lead, geometry = _visible_checks(q, k_cache, v_cache, out, query_start_loc, seq_lens, block_table, window, sinks)
+    _kv_scales_check(kv_scales, k_cache)
+    return _decode_visible("fp8kv_decode_attn_blk", q, out, lead, (kv_scales.data_ptr(),), sm_scale, geometry, seq_lens,
+                           window, sinks, num_splits, max_seq_len, scratch, False)
+
+
+def prefill_attention_blk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor,
+                          cu_seqlens_q: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor,
+                          kv_scales: torch.Tensor, sm_scale: float, window: int = 0, sinks: int = 0,
+                          max_query_len: int | None = None) -> torch.Tensor:
+    """``prefill_attention_varlen`` over the block-scaled e4m3 cache that ``rope_append_blk`` writes, with ``window``
+    and ``sinks`` as in ``prefill_attention_window``."""
+    _fp8_cache_check(k_cache, "k_cache")
+    _fp8_cache_check(v_cache, "v_cache")
+    lead, geometry = _visible_checks(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, window, sinks)
+    _kv_scales_check(kv_scales, k_cache)
+    return _prefill_visible("fp8kv_prefill_attn_blk", q, out, lead, (kv_scales.data_ptr(),), sm_scale, geometry,
+                            cu_seqlens_q, window, sinks, max_query_len)
+
+
 # ------------------------------------------------------------------------------ layer epilogues
 
 def _bf16_rows(t: torch.Tensor, name: str) -> None:

@@ -281,6 +281,100 @@ int fp8kv_prefill_attn_varlen_bf16(const void* q, int64_t q_row_stride,
                                    int block_size, int max_query_len, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Attention with a sliding window and a few first tokens that stay visible (sinks).
+ *
+ *   The query at position p of its sequence sees the keys t <= p with t > p - window or t < sinks; window 0: all
+ *   keys t <= p (sinks then say nothing).  window, sinks >= 0.
+ *
+ * decode: one query per sequence, at position seq_lens[s] - 1; prefill: the packed sequences of
+ * fp8kv_prefill_attn_varlen, row i of sequence s at position seq_lens[s] - qlen_s + i.  Layouts, strides, geometry limits,
+ * splits, scratch and max_seq_len as for fp8kv_decode_attn_ctx and fp8kv_prefill_attn_varlen (bf16: as for their bf16
+ * forms); fp8kv_decode_num_splits is asked with the longest visible set, min(max_seq_len, window + sinks).
+ *   - Block-table entries of blocks without a visible key are never used, whatever they hold, so blocks that the
+ *     window has left can be given back.
+ *   - Rows that see nothing are zeros: seq_lens[s] <= 0, and rows of negative position (seq_lens[s] < qlen_s).
+ *   - Keys that a row does not see do not reach it, whatever they hold (a NaN or an infinity included); a
+ *     non-finite element of a key that it sees reaches that element of its output.
+ * The probabilities enter P.V in more than bf16's precision (decode: bf16 hi + lo parts; prefill: fp16 over e4m3
+ * caches); prefill over bf16 caches rounds them to bf16 and sums the rounded values.
+ * No counterpart in the reference, whose hook leaves such layers to stock vLLM (vllm-fp8kv/fp8kv_override.py:50-64). */
+int fp8kv_decode_attn_window(const void* q, int64_t q_row_stride,
+                             const void* k_cache, const void* v_cache,
+                             int64_t sk0, int64_t sk1, int64_t sk2,
+                             int64_t sv0, int64_t sv1, int64_t sv2,
+                             void* out, int64_t out_row_stride,
+                             const int32_t* query_start_loc, const int32_t* seq_lens,
+                             const int32_t* block_table, int64_t bt_stride,
+                             const float* k_scale, const float* v_scale, float sm_scale,
+                             int num_seqs, int num_q_heads, int num_kv_heads, int head_size,
+                             int block_size, int num_splits, void* scratch, size_t scratch_bytes,
+                             int window, int sinks, int max_seq_len, void* stream);
+
+int fp8kv_decode_attn_window_bf16(const void* q, int64_t q_row_stride,
+                                  const void* k_cache, const void* v_cache,
+                                  int64_t sk0, int64_t sk1, int64_t sk2,
+                                  int64_t sv0, int64_t sv1, int64_t sv2,
+                                  void* out, int64_t out_row_stride,
+                                  const int32_t* query_start_loc, const int32_t* seq_lens,
+                                  const int32_t* block_table, int64_t bt_stride,
+                                  float sm_scale,
+                                  int num_seqs, int num_q_heads, int num_kv_heads, int head_size,
+                                  int block_size, int num_splits, void* scratch, size_t scratch_bytes,
+                                  int window, int sinks, int max_seq_len, void* stream);
+
+int fp8kv_prefill_attn_window(const void* q, int64_t q_row_stride,
+                              const void* k_cache, const void* v_cache,
+                              int64_t sk0, int64_t sk1, int64_t sk2,
+                              int64_t sv0, int64_t sv1, int64_t sv2,
+                              void* out, int64_t out_row_stride,
+                              const int32_t* cu_seqlens_q, const int32_t* seq_lens,
+                              const int32_t* block_table, int64_t bt_stride,
+                              const float* k_scale, const float* v_scale, float sm_scale,
+                              int num_seqs, int num_q_heads, int num_kv_heads, int head_size,
+                              int block_size, int window, int sinks, int max_query_len, void* stream);
+
+int fp8kv_prefill_attn_window_bf16(const void* q, int64_t q_row_stride,
+                                   const void* k_cache, const void* v_cache,
+                                   int64_t sk0, int64_t sk1, int64_t sk2,
+                                   int64_t sv0, int64_t sv1, int64_t sv2,
+                                   void* out, int64_t out_row_stride,
+                                   const int32_t* cu_seqlens_q, const int32_t* seq_lens,
+                                   const int32_t* block_table, int64_t bt_stride,
+                                   float sm_scale,
+                                   int num_seqs, int num_q_heads, int num_kv_heads, int head_size,
+                                   int block_size, int window, int sinks, int max_query_len, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Attention over a block-scaled cache (fp8kv_rope_append_blk): e4m3 codes with one power-of-two scale per 16
+ * tokens, kv head and tensor,
+ *   K_t = code * 2^(b_K - 127), V_t = code * 2^(b_V - 127), b = kv_scales[block][slot / 16][kv head],
+ * kv_scales uint8 [blocks, block_size / 16, num_kv_heads, 2] contiguous, 2-byte aligned, bytes below 255.  With
+ * window and sinks as above (0, 0: whole causal contexts); everything else, the guarantees too, as there.
+ * No counterpart in the reference. */
+int fp8kv_decode_attn_blk(const void* q, int64_t q_row_stride,
+                          const void* k_cache, const void* v_cache,
+                          int64_t sk0, int64_t sk1, int64_t sk2,
+                          int64_t sv0, int64_t sv1, int64_t sv2,
+                          void* out, int64_t out_row_stride,
+                          const int32_t* query_start_loc, const int32_t* seq_lens,
+                          const int32_t* block_table, int64_t bt_stride,
+                          const void* kv_scales, float sm_scale,
+                          int num_seqs, int num_q_heads, int num_kv_heads, int head_size,
+                          int block_size, int num_splits, void* scratch, size_t scratch_bytes,
+                          int window, int sinks, int max_seq_len, void* stream);
+
+int fp8kv_prefill_attn_blk(const void* q, int64_t q_row_stride,
+                           const void* k_cache, const void* v_cache,
+                           int64_t sk0, int64_t sk1, int64_t sk2,
+                           int64_t sv0, int64_t sv1, int64_t sv2,
+                           void* out, int64_t out_row_stride,
+                           const int32_t* cu_seqlens_q, const int32_t* seq_lens,
+                           const int32_t* block_table, int64_t bt_stride,
+                           const void* kv_scales, float sm_scale,
+                           int num_seqs, int num_q_heads, int num_kv_heads, int head_size,
+                           int block_size, int window, int sinks, int max_query_len, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * fp8-e4m3 KV-cache write: quantise new K and V rows and scatter them into the paged cache.
  *
  *   k_cache[block, slot, h, d] = e4m3fn( float(key[i, h, d]) / k_scale )   (V likewise)

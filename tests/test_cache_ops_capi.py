@@ -1,8 +1,10 @@
-"""Argument rejection of the append calls, before any launch (no GPU; the pointers are never followed)."""
+"""Argument rejection of the append and visible-key attention calls, before any launch (no GPU; the pointers are
+never followed), and checks of their oracles."""
 import numpy as np
 import pytest
+import torch
 
-from oracle import formats, rope_append
+from oracle import attention, formats, rope_append, visible
 
 A = 0x10000
 # q, q_out, key, value with strides, caches, strides (engine layout of 4 kv heads, blocks of 16), rotation
@@ -70,6 +72,70 @@ def test_append_of_nothing_is_a_no_op(lib):
                                  16, 100, None) == 0
 
 
+# q .. bt_stride of the attention calls: 24 / 4 heads, the engine's layout with blocks of 16
+ATT = [A, 24 * 128, A, A + 128, 16384, 256, 4096, 16384, 256, 4096, A, 24 * 128, A, A, A, 64]
+GEO = [8, 24, 4, 128, 16]
+
+
+def _att(elem=1, **at):
+    args = list(ATT)
+    if elem == 2:
+        args[3] = A + 256
+    for i, v in at.items():
+        args[int(i[1:])] = v
+    return args
+
+
+ATT_CHECKS = [(dict(_0=None), 1), (dict(_2=None), 1), (dict(_10=None), 1), (dict(_12=None), 1), (dict(_13=None), 1),
+              (dict(_14=None), 1), (dict(_15=-1), 1), (dict(_0=A + 8), 3), (dict(_2=A + 8), 3), (dict(_3=A + 4), 3), (dict(_1=3076), 3),
+              (dict(_5=264), 3), (dict(_8=260), 3), (dict(_5=-256), 2)]
+GEO_CHECKS = [([0, 24, 4, 128, 16], 1), ([8, 0, 4, 128, 16], 1), ([8, 24, 0, 128, 16], 1), ([8, 25, 4, 128, 16], 2), ([8, 68, 4, 128, 16], 2),
+              ([8, 24, 4, 64, 16], 2), ([8, 24, 4, 128, 8], 2), ([8, 24, 4, 128, 48], 2), ([65536, 24, 4, 128, 16], 2)]
+
+
+def _forms(lib):
+    """(decode call, prefill call, element bytes, scale arguments) of every cache kind."""
+    return ((lib.fp8kv_decode_attn_window, lib.fp8kv_prefill_attn_window, 1, [A, A]),
+            (lib.fp8kv_decode_attn_window_bf16, lib.fp8kv_prefill_attn_window_bf16, 2, []),
+            (lib.fp8kv_decode_attn_blk, lib.fp8kv_prefill_attn_blk, 1, [A]))
+
+
+@pytest.mark.parametrize("change,code", ATT_CHECKS)
+def test_visible_attention_rejects_before_launch(lib, change, code):
+    for dec, pre, elem, scales in _forms(lib):
+        if elem == 2 and "_5" in change and change["_5"] == 264:
+            change = dict(_5=260)
+        args = _att(elem, **change)
+        assert dec(*args, *scales, 0.1, *GEO, 4, None, 0, 64, 4, 0, None) == code
+        assert pre(*args, *scales, 0.1, *GEO, 64, 4, 0, None) == code
+
+
+@pytest.mark.parametrize("geo,code", GEO_CHECKS)
+def test_visible_attention_geometry(lib, geo, code):
+    for dec, pre, elem, scales in _forms(lib):
+        assert dec(*_att(elem), *scales, 0.1, *geo, 4, None, 0, 64, 4, 0, None) == code
+        assert pre(*_att(elem), *scales, 0.1, *geo, 64, 4, 0, None) == code
+
+
+def test_visible_attention_window_splits_and_scales(lib):
+    for dec, pre, elem, scales in _forms(lib):
+        args = _att(elem)
+        for win in ((-1, 0), (0, -1)):
+            assert dec(*args, *scales, 0.1, *GEO, 1, None, 0, *win, 0, None) == 1
+            assert pre(*args, *scales, 0.1, *GEO, *win, 0, None) == 1
+        assert dec(*args, *scales, 0.1, *GEO, 0, None, 0, 64, 4, 0, None) == 1
+        assert dec(*args, *scales, 0.1, *GEO, 257, None, 0, 64, 4, 0, None) == 1
+        assert dec(*args, *scales, 0.1, *GEO, 4, A, 100, 64, 4, 0, None) == 5
+        assert pre(*args, *scales, 0.1, *GEO, 64, 4, -1, None) == 1
+        for i in range(len(scales)):
+            missing = scales[:i] + [None] + scales[i + 1:]
+            assert dec(*args, *missing, 0.1, *GEO, 1, None, 0, 64, 4, 0, None) == 1
+            assert pre(*args, *missing, 0.1, *GEO, 64, 4, 0, None) == 1
+        assert pre(*args, *scales, 0.1, *GEO, 64, 4, 0, None) == 0                    # no queries: nothing is launched
+    assert lib.fp8kv_decode_attn_blk(*_att(), A + 1, 0.1, *GEO, 1, None, 0, 64, 4, 0, None) == 3
+    assert lib.fp8kv_prefill_attn_blk(*_att(), A + 1, 0.1, *GEO, 64, 4, 0, None) == 3
+
+
 # ---- the oracle itself ---------------------------------------------------------------------------
 
 def test_oracle_rotation_keeps_norms_and_composes():
@@ -98,3 +164,33 @@ def test_oracle_exponents_and_rounding():
     mids = (np.sort(np.unique(fine))[1:] + np.sort(np.unique(fine))[:-1]) / 2
     from oracle.kv_cache import encode_e4m3fn_satfinite
     assert np.array_equal(rope_append.round_e4m3(mids), codes[encode_e4m3fn_satfinite(mids.astype(np.float32))])
+
+
+def test_oracle_visible_keys():
+    assert visible.visible(9, 10, 0, 3).tolist() == list(range(10))
+    assert visible.visible(9, 10, 4, 2).tolist() == [0, 1, 6, 7, 8, 9]
+    assert visible.visible(9, 10, 1, 0).tolist() == [9]
+    assert visible.visible(2, 10, 5, 9).tolist() == [0, 1, 2]
+    assert visible.visible(-1, 10, 5, 9).numel() == 0 and visible.visible(4, 0, 0, 0).numel() == 0
+
+
+def test_oracle_agrees_with_the_whole_context_oracle_and_with_masked_softmax():
+    from fp8kv_amd import workloads
+    c = workloads.prefill_case([9, 4], [20, 0], HQ=4, HKV=2, seed=1)
+    args = (c["q"], c["k_cache"], c["v_cache"], c["cu_seqlens_q"], c["seq_lens"], c["block_table"], c["k_scale"], c["v_scale"], c["sm_scale"])
+    whole = attention.varlen_prefill_attention(*args)
+    assert torch.allclose(visible.attention(*args)[0], whole, atol=1e-12)
+    assert torch.allclose(visible.attention(*args, window=100, sinks=3)[0], whole, atol=1e-12)
+    got = visible.attention(*args, window=6, sinks=2)[0]
+    k, v = (attention.gather_kv(c[n], c["block_table"][0], 29, 1) for n in ("k_cache", "v_cache"))
+    for i in range(9):
+        p = 20 + i
+        hidden = torch.tensor([t > p or (t <= p - 6 and t >= 2) for t in range(29)])
+        s = (c["q"][i, 3].double() @ k.T * c["sm_scale"] * c["k_scale"]).masked_fill(hidden, -float("inf"))
+        assert torch.allclose(got[i, 3], torch.softmax(s, -1) @ v * c["v_scale"], atol=1e-12)
+    # scales that are powers of two: the block-scaled form of the same values
+    sc = torch.full((c["k_cache"].shape[0], 1, 2, 2), 127, dtype=torch.uint8)
+    sc[..., 0] += 3
+    a = visible.attention(*args[:6], (sc, 0), (sc, 1), c["sm_scale"], 6, 2)[0]
+    b = visible.attention(*args[:6], 8.0, 1.0, c["sm_scale"], 6, 2)[0]
+    assert torch.allclose(a, b, atol=1e-12)
