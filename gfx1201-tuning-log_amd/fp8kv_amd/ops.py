@@ -383,60 +383,104 @@ def rope_table(num_positions: int, rotary_dim: int, device, base: float = 10000.
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_BF16, _E4M3, _U8, _I32, _I64, _F32 = (torch.bfloat16, torch.float8_e4m3fn, torch.uint8, torch.int32, torch.int64,
+                                       torch.float32)
+_E8M0 = torch.float8_e8m0fnu
 
 
-def _launch(name: str, t: torch.Tensor, *args) -> None:
-    """Entry point ``name`` on the current stream of ``t``'s device, whichever device is current."""
+# The calls below run once per layer and step, like those above, and take a dozen tensors each.  Every property that is
+# read of a tensor costs about 0.1 us, so each is read once: shape and stride as whole tuples, the device as its number
+# (-1 on the CPU).
+def _launch(name: str, dev: int, *args) -> None:
+    """Entry point ``name`` on the current stream of device ``dev``, whichever device is current."""
     fn = getattr(_lib.load(), name)
-    if t.device.index == _current_device():
-        st = fn(*args, _stream_ptr(t))
+    if dev == _current_device():
+        st = fn(*args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream)
     else:
-        with torch.cuda.device(t.device):
-            st = fn(*args, _stream_ptr(t))
-    _lib.check(name, st)
+        with torch.cuda.device(dev):
+            st = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if st != 0:
+        _lib.check(name, st)
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements between the token rows of [T, H, D] (a single row's stride says nothing)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+def _heads(t: torch.Tensor, name: str) -> tuple:
+    """(T, H, D, elements between the rows, device) of a bf16 [T, H, D] tensor whose heads are contiguous.  A
+    single row's stride says nothing and is replaced."""
+    shape, stride, dev = t.shape, t.stride(), t.get_device()
+    if not (len(shape) == 3 and t.dtype is _BF16 and dev >= 0 and stride[2] == 1 and (stride[1] == shape[2] or shape[1] == 1)):
+        raise ValueError(f"{name} must be a bf16 device tensor [T, heads, D] with contiguous heads")
+    return shape[0], shape[1], shape[2], stride[0] if shape[0] > 1 else shape[1] * shape[2], dev
 
 
-def _rope_args(q, key, value, k_cache, v_cache, positions, cos_sin, q_out, interleaved):
-    """Checks what the append calls share; (q_out, leading arguments of the C calls)."""
-    T, HKV, D = key.shape if key.dim() == 3 else (0, 0, 0)
-    for t, n in ((key, "key"), (value, "value")):
-        if not (t.is_cuda and t.dtype == torch.bfloat16 and t.dim() == 3 and t.shape == key.shape and
-                t.stride(2) == 1 and (t.stride(1) == D or HKV == 1)):
-            raise ValueError(f"{n} must be bf16 [T, HKV, D] with contiguous heads (key and value of one shape)")
-    dev = key.device
-    if not (k_cache.shape == v_cache.shape and k_cache.shape[2] == HKV and k_cache.shape[3] == D):
-        raise ValueError("caches must be [NB, PBLK, HKV, D] matching key")
-    if not (value.device == k_cache.device == v_cache.device == dev):
+def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: int, D: int, allow_bf16: bool) -> tuple:
+    """(is bf16, NB, PBLK, HKV, addresses and strides as the C calls take them) of a cache's K and V views."""
+    kd, vd = k_cache.dtype, v_cache.dtype
+    bf16 = kd is _BF16 and vd is _BF16
+    if not (bf16 and allow_bf16) and not ((kd is _E4M3 or kd is _U8) and (vd is _E4M3 or vd is _U8)):
+        raise ValueError("caches must both be e4m3 (float8_e4m3fn or raw uint8)" + (" or both bf16" if allow_bf16 else ""))
+    ks, vs = k_cache.stride(), v_cache.stride()
+    shape = k_cache.shape
+    if not (len(shape) == 4 and shape == v_cache.shape and shape[3] == D and ks[3] == 1 and vs[3] == 1):
+        raise ValueError("caches must be [NB, PBLK, HKV, D] of one shape, contiguous along the head size that q and key have")
+    if not (k_cache.get_device() == dev and v_cache.get_device() == dev):
         raise ValueError("tensors on different devices")
-    q_args = (None, 0, None, 0)
+    return bf16, shape[0], shape[1], shape[2], (k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2],
+                                                vs[0], vs[1], vs[2])
+
+
+def _vector(t: torch.Tensor, name: str, dtype, n: int, dev: int) -> int:
+    """Address of a contiguous vector of n elements."""
+    shape = t.shape
+    if not (t.dtype is dtype and len(shape) == 1 and shape[0] == n and t.is_contiguous() and t.get_device() == dev):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor [{n}] on device {dev}")
+    return t.data_ptr()
+
+
+def _sequences(starts: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, dev: int) -> tuple:
+    """(NS, max_blocks, addresses and stride) of the sequences' metadata."""
+    shape, stride = block_table.shape, block_table.stride()
+    if not (len(shape) == 2 and block_table.dtype is _I32 and (stride[1] == 1 or shape[1] <= 1) and
+            block_table.get_device() == dev):
+        raise ValueError(f"block_table must be an int32 tensor [NS, max_blocks] on device {dev}, rows contiguous")
+    return shape[0], shape[1], (_vector(starts, "query_start_loc", _I32, shape[0] + 1, dev),
+                                _vector(seq_lens, "seq_lens", _I32, shape[0], dev), block_table.data_ptr(), stride[0])
+
+
+def _kv_scales(t: torch.Tensor, NB: int, PBLK: int, HKV: int, dev: int) -> int:
+    if not ((t.dtype is _U8 or t.dtype is _E8M0) and t.shape == (NB, PBLK // 16, HKV, 2) and t.is_contiguous() and
+            t.get_device() == dev):
+        raise ValueError(f"kv_scales must be contiguous uint8 (e8m0) [{NB}, {PBLK // 16}, {HKV}, 2] on device {dev}")
+    return t.data_ptr()
+
+
+def _rope_args(q, key, value, positions, cos_sin, q_out, interleaved):
+    """Checks what the append calls share; (q_out, T, HQ, HKV, D, device, arguments of queries, keys, values, rotation)."""
+    T, HKV, D, k_stride, dev = _heads(key, "key")
+    vT, vH, vD, v_stride, v_dev = _heads(value, "value")
+    if not (vT == T and vH == HKV and vD == D and v_dev == dev):
+        raise ValueError("key and value must have the same shape and device")
+    HQ, q_args = 0, (None, 0, None, 0)
     if q is not None:
+        qT, HQ, qD, q_stride, q_dev = _heads(q, "q")
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        for t, n in ((q, "q"), (q_out, "q_out")):
-            if not (t.dtype == torch.bfloat16 and t.dim() == 3 and t.device == dev and t.shape == q.shape and
-                    t.shape[0] == T and t.shape[2] == D and t.stride(2) == 1 and (t.stride(1) == D or t.shape[1] == 1)):
-                raise ValueError(f"{n} must be bf16 [T, HQ, D] with contiguous heads on key's device")
-        q_args = (q.data_ptr(), _row_stride(q), q_out.data_ptr(), _row_stride(q_out))
+            q_out = torch.empty((qT, HQ, qD), dtype=_BF16, device=q.device)
+        oT, oH, oD, o_stride, o_dev = _heads(q_out, "q_out")
+        if not (qT == oT == T and oH == HQ and qD == oD == D and q_dev == o_dev == dev):
+            raise ValueError("q and q_out must be [T, HQ, D] of key's T, D and device")
+        q_args = (q.data_ptr(), q_stride, q_out.data_ptr(), o_stride)
     elif q_out is not None:
         raise ValueError("q_out without q")
     table = (None, None, 0, 0, 0, 0, 0)
     if cos_sin is not None:
-        if not (cos_sin.dim() == 2 and cos_sin.dtype in (torch.float32, torch.bfloat16) and cos_sin.stride(1) == 1 and
-                cos_sin.device == dev):
+        shape, stride, dtype = cos_sin.shape, cos_sin.stride(), cos_sin.dtype
+        if not (len(shape) == 2 and (dtype is _F32 or dtype is _BF16) and stride[1] == 1 and cos_sin.get_device() == dev):
             raise ValueError("cos_sin must be fp32 or bf16 [positions, rotary_dim] on key's device")
-        if not (positions is not None and positions.dtype == torch.int64 and positions.shape == (T,) and
-                positions.is_contiguous() and positions.device == dev):
-            raise ValueError("positions must be a contiguous int64 device tensor [T]")
-        table = (positions.data_ptr(), cos_sin.data_ptr(), cos_sin.stride(0), int(cos_sin.dtype == torch.bfloat16),
-                 cos_sin.shape[0], cos_sin.shape[1], int(bool(interleaved)))
-    return q_out, (*q_args, key.data_ptr(), _row_stride(key), value.data_ptr(), _row_stride(value),
-                   k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-                   v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), *table)
+        if positions is None:
+            raise ValueError("cos_sin without positions")
+        table = (_vector(positions, "positions", _I64, T, dev), cos_sin.data_ptr(),
+                 stride[0] if shape[0] > 1 else shape[1], 1 if dtype is _BF16 else 0, shape[0], shape[1],
+                 1 if interleaved else 0)
+    return q_out, T, HQ, HKV, D, dev, (*q_args, key.data_ptr(), k_stride, value.data_ptr(), v_stride), table
 
 
 def rope_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -451,31 +495,21 @@ def rope_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor, 
     (``rope_table``); the first R elements of a head are rotated, paired in halves or, ``interleaved``,
     adjacent.  A position outside the table gives NaN.  ``cos_sin=None``: no rotation; ``q=None``: keys and
     values only.  fp32 arithmetic, rounded once (fp8kv_rope_append)."""
-    bf16_kv = _kv_caches_bf16(k_cache, v_cache)
-    q_out, args = _rope_args(q, key, value, k_cache, v_cache, positions, cos_sin, q_out, interleaved)
-    T, HKV, D = key.shape
-    dev = key.device
-    if not (slot_mapping.dtype == torch.int64 and slot_mapping.shape == (T,) and slot_mapping.is_contiguous() and
-            slot_mapping.device == dev):
-        raise ValueError("slot_mapping must be a contiguous int64 device tensor [T]")
+    q_out, T, HQ, HKV, D, dev, rows, table = _rope_args(q, key, value, positions, cos_sin, q_out, interleaved)
+    bf16_kv, NB, PBLK, cH, caches = _caches(k_cache, v_cache, dev, D, True)
+    if cH != HKV:
+        raise ValueError("caches must be [NB, PBLK, HKV, D] matching key")
+    slots = _vector(slot_mapping, "slot_mapping", _I64, T, dev)
     if bf16_kv:
-        name, scales = "fp8kv_rope_append_bf16", ()
-    else:
-        if k_scale is None or v_scale is None:
-            raise ValueError("e4m3 caches need k_scale and v_scale")
-        ks, vs = _scale_tensor(k_scale, dev), _scale_tensor(v_scale, dev)
-        name, scales = "fp8kv_rope_append", (ks.data_ptr(), vs.data_ptr())
+        if T > 0:
+            _launch("fp8kv_rope_append_bf16", dev, *rows, *caches, *table, slots, T, HQ, HKV, D, PBLK, NB)
+        return q_out
+    if k_scale is None or v_scale is None:
+        raise ValueError("e4m3 caches need k_scale and v_scale")
+    ks, vs = _scale_tensor(k_scale, key.device), _scale_tensor(v_scale, key.device)
     if T > 0:
-        _launch(name, key, *args, slot_mapping.data_ptr(), *scales, T, 0 if q is None else q.shape[1], HKV, D,
-                k_cache.shape[1], k_cache.shape[0])
+        _launch("fp8kv_rope_append", dev, *rows, *caches, *table, slots, ks.data_ptr(), vs.data_ptr(), T, HQ, HKV, D, PBLK, NB)
     return q_out
-
-
-def _kv_scales_check(kv_scales: torch.Tensor, k_cache: torch.Tensor) -> None:
-    NB, PBLK, HKV = k_cache.shape[:3]
-    if not (kv_scales.dtype in (torch.uint8, torch.float8_e8m0fnu) and kv_scales.device == k_cache.device and
-            kv_scales.shape == (NB, PBLK // 16, HKV, 2) and kv_scales.is_contiguous()):
-        raise ValueError(f"kv_scales must be contiguous uint8 (e8m0) [{NB}, {PBLK // 16}, {HKV}, 2] on the caches' device")
 
 
 def rope_append_blk(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -491,93 +525,50 @@ def rope_append_blk(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tens
     row s (int32 device tensors, the metadata of the attention calls).  A group of 16 that also holds
     earlier tokens keeps its scale unless the new ones need a larger one; then the old codes are re-rounded.
     Rows of q_out behind the last sequence are left as they were (fp8kv_rope_append_blk)."""
-    _fp8_cache_check(k_cache, "k_cache")
-    _fp8_cache_check(v_cache, "v_cache")
-    q_out, args = _rope_args(q, key, value, k_cache, v_cache, positions, cos_sin, q_out, interleaved)
-    T, HKV, D = key.shape
-    dev = key.device
-    _kv_scales_check(kv_scales, k_cache)
-    for t, n in ((query_start_loc, "query_start_loc"), (seq_lens, "seq_lens"), (block_table, "block_table")):
-        if not (t.dtype == torch.int32 and t.device == dev and (t.stride(-1) == 1 or t.shape[-1] == 1)):
-            raise ValueError(f"{n} must be an int32 tensor on key's device, contiguous along its last axis")
-    if not (block_table.dim() == 2 and query_start_loc.shape == (block_table.shape[0] + 1,) and
-            seq_lens.shape == (block_table.shape[0],)):
-        raise ValueError("block_table must be [NS, max_blocks], query_start_loc [NS + 1], seq_lens [NS]")
-    if T > 0 and block_table.shape[0] > 0:
-        _launch("fp8kv_rope_append_blk", key, *args, kv_scales.data_ptr(), query_start_loc.data_ptr(),
-                seq_lens.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-                block_table.shape[0], T, 0 if q is None else q.shape[1], HKV, D, k_cache.shape[1], k_cache.shape[0])
+    q_out, T, HQ, HKV, D, dev, rows, table = _rope_args(q, key, value, positions, cos_sin, q_out, interleaved)
+    _, NB, PBLK, cH, caches = _caches(k_cache, v_cache, dev, D, False)
+    if cH != HKV:
+        raise ValueError("caches must be [NB, PBLK, HKV, D] matching key")
+    scales = _kv_scales(kv_scales, NB, PBLK, HKV, dev)
+    NS, max_blocks, seqs = _sequences(query_start_loc, seq_lens, block_table, dev)
+    if T > 0 and NS > 0:
+        _launch("fp8kv_rope_append_blk", dev, *rows, *caches, *table, scales, *seqs, max_blocks, NS, T, HQ, HKV, D, PBLK, NB)
     return q_out
 
 
 # ------------------------------------------------------------------------------ attention over visible keys
 
-def _visible_checks(q, k_cache, v_cache, out, starts, seq_lens, block_table, window, sinks):
-    """Checks what the calls below share; (leading arguments, trailing geometry) of the C calls."""
-    T, HQ, D = q.shape if q.dim() == 3 else (0, 0, 0)
-    for t, n in ((q, "q"), (out, "out")):
-        if not (t.dtype == torch.bfloat16 and t.dim() == 3 and t.is_cuda and t.stride(2) == 1 and
-                (t.stride(1) == D or HQ == 1) and t.shape[1:] == q.shape[1:]):
-            raise ValueError(f"{n} must be bf16 [T, HQ, D] with contiguous heads")
-    dev = q.device
-    if not (k_cache.shape == v_cache.shape and k_cache.shape[3] == D):
-        raise ValueError("caches must be [NB, PBLK, HKV, D] of q's head size")
-    for t, n in ((starts, "query_start_loc"), (seq_lens, "seq_lens"), (block_table, "block_table")):
-        if not (t.dtype == torch.int32 and t.device == dev and (t.stride(-1) == 1 or t.shape[-1] == 1)):
-            raise ValueError(f"{n} must be an int32 tensor on q's device, contiguous along its last axis")
-    NS = block_table.shape[0]
-    if not (block_table.dim() == 2 and starts.shape == (NS + 1,) and seq_lens.shape == (NS,)):
-        raise ValueError("block_table must be [NS, max_blocks], query_start_loc [NS + 1], seq_lens [NS]")
-    if not (out.device == k_cache.device == v_cache.device == dev):
-        raise ValueError("tensors on different devices")
-    if not (window >= 0 and sinks >= 0):
+def _attention_args(q, k_cache, v_cache, out, starts, seq_lens, block_table, window, sinks, allow_bf16):
+    """Checks what the calls below share; (device, is bf16, leading arguments, trailing geometry) of the C calls."""
+    _, HQ, D, q_stride, dev = _heads(q, "q")
+    _, oH, oD, o_stride, o_dev = _heads(out, "out")
+    if not (oH == HQ and oD == D and o_dev == dev):
+        raise ValueError("out must be [T, HQ, D] of q's heads and device")
+    bf16, NB, PBLK, HKV, caches = _caches(k_cache, v_cache, dev, D, allow_bf16)
+    NS, _, seqs = _sequences(starts, seq_lens, block_table, dev)
+    if window < 0 or sinks < 0:
         raise ValueError("window and sinks must not be negative")
-    lead = (q.data_ptr(), _row_stride(q), k_cache.data_ptr(), v_cache.data_ptr(),
-            k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-            v_cache.stride(0), v_cache.stride(1), v_cache.stride(2),
-            out.data_ptr(), _row_stride(out), starts.data_ptr(), seq_lens.data_ptr(),
-            block_table.data_ptr(), block_table.stride(0))
-    return lead, (NS, HQ, k_cache.shape[2], D, k_cache.shape[1])
+    return dev, bf16, (q.data_ptr(), q_stride, *caches, out.data_ptr(), o_stride, *seqs), (NS, HQ, HKV, D, PBLK), NB
 
 
-def _decode_visible(name, q, out, lead, scales, sm_scale, geometry, seq_lens, window, sinks, num_splits, max_seq_len,
-                    scratch, bf16_kv):
+def _decode_visible(name, dev, lead, scales, sm_scale, geometry, q, seq_lens, window, sinks, num_splits, max_seq_len, scratch,
+                    bf16_kv):
     NS, HQ, HKV, D, _ = geometry
-    if NS == 0:
-        return out
     if num_splits is None:
-        if max_seq_len is None and window == 0:
-            max_seq_len = int(seq_lens.max().item())
-        visible = window + sinks if max_seq_len is None else max_seq_len
         if window > 0:
-            visible = min(visible, window + sinks)
+            visible = window + sinks if max_seq_len is None else min(max_seq_len, window + sinks)
+        else:
+            if max_seq_len is None:
+                max_seq_len = int(seq_lens.max().item())
+            visible = max_seq_len
         num_splits = decode_num_splits(NS, HKV, min(int(visible), 1 << 30), bf16_kv)
-    need = decode_scratch_bytes(NS, HQ, HKV, num_splits, D)
+    need = decode_scratch_bytes(NS, HQ, HKV, num_splits, D) if num_splits > 1 else 0
     if scratch is None:
         scratch = _call_scratch(need, q.device)
-    elif need > 0:
-        if not (scratch.is_cuda and scratch.numel() * scratch.element_size() >= need):
-            raise ValueError(f"scratch needs {need} bytes")
-    sbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
-    _launch(name, q, *lead, *scales, float(sm_scale), *geometry, int(num_splits), _ptr(scratch), sbytes, int(window),
-            int(sinks), int(max_seq_len or 0))
-    return out
-
-
-def _prefill_visible(name, q, out, lead, scales, sm_scale, geometry, starts, window, sinks, max_query_len):
-    if max_query_len is None:
-        max_query_len = int((starts[1:] - starts[:-1]).max().item()) if geometry[0] else 0
-    if q.shape[0] > 0 and geometry[0] > 0:
-        _launch(name, q, *lead, *scales, float(sm_scale), *geometry, int(window), int(sinks), int(max_query_len))
-    return out
-
-
-def _per_tensor_scales(k_cache, v_cache, k_scale, v_scale, dev):
-    """(suffix of the entry point, its scale arguments, tensors that must live until the launch)."""
-    if _kv_caches_bf16(k_cache, v_cache):
-        return "_bf16", (), ()
-    ks, vs = _scale_tensor(k_scale, dev), _scale_tensor(v_scale, dev)
-    return "", (ks.data_ptr(), vs.data_ptr()), (ks, vs)
+    elif not (scratch.get_device() == dev and scratch.numel() * scratch.element_size() >= need):
+        raise ValueError(f"scratch needs {need} bytes on device {dev}")
+    where, sbytes = (None, 0) if scratch is None else (scratch.data_ptr(), scratch.numel() * scratch.element_size())
+    _launch(name, dev, *lead, *scales, sm_scale, *geometry, num_splits, where, sbytes, window, sinks, max_seq_len or 0)
 
 
 def decode_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor,
@@ -590,10 +581,17 @@ def decode_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
     Only the visible keys are read; block-table entries of blocks that hold none may be anything.  A window bounds
     the work, so ``max_seq_len`` is needed only without one (and then read from ``seq_lens``, which synchronises)."""
-    suffix, scales, keep = _per_tensor_scales(k_cache, v_cache, k_scale, v_scale, q.device)
-    lead, geometry = _visible_checks(q, k_cache, v_cache, out, query_start_loc, seq_lens, block_table, window, sinks)
-    return _decode_visible("fp8kv_decode_attn_window" + suffix, q, out, lead, scales, sm_scale, geometry, seq_lens, window,
-                           sinks, num_splits, max_seq_len, scratch, suffix == "_bf16")
+    dev, bf16, lead, geometry, _ = _attention_args(q, k_cache, v_cache, out, query_start_loc, seq_lens, block_table, window,
+                                                   sinks, True)
+    if geometry[0] == 0:
+        return out
+    name, scales = "fp8kv_decode_attn_window_bf16", ()
+    if not bf16:
+        ks, vs = _scale_tensor(k_scale, q.device), _scale_tensor(v_scale, q.device)
+        name, scales = "fp8kv_decode_attn_window", (ks.data_ptr(), vs.data_ptr())
+    _decode_visible(name, dev, lead, scales, sm_scale, geometry, q, seq_lens, window, sinks, num_splits, max_seq_len, scratch,
+                    bf16)
+    return out
 
 
 def prefill_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor,
@@ -602,10 +600,19 @@ def prefill_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
                              max_query_len: int | None = None) -> torch.Tensor:
     """``prefill_attention_varlen`` where the query at position p sees the keys t <= p with t > p - window
     or t < sinks (window 0: all t <= p).  Caches e4m3 with per-tensor scales, or bf16."""
-    suffix, scales, keep = _per_tensor_scales(k_cache, v_cache, k_scale, v_scale, q.device)
-    lead, geometry = _visible_checks(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, window, sinks)
-    return _prefill_visible("fp8kv_prefill_attn_window" + suffix, q, out, lead, scales, sm_scale, geometry, cu_seqlens_q,
-                            window, sinks, max_query_len)
+    dev, bf16, lead, geometry, _ = _attention_args(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, window,
+                                                   sinks, True)
+    if geometry[0] == 0 or q.shape[0] == 0:
+        return out
+    if max_query_len is None:
+        max_query_len = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item())
+    if bf16:
+        _launch("fp8kv_prefill_attn_window_bf16", dev, *lead, sm_scale, *geometry, window, sinks, max_query_len)
+    else:
+        ks, vs = _scale_tensor(k_scale, q.device), _scale_tensor(v_scale, q.device)
+        _launch("fp8kv_prefill_attn_window", dev, *lead, ks.data_ptr(), vs.data_ptr(), sm_scale, *geometry, window, sinks,
+                max_query_len)
+    return out
 
 
 def decode_attention_blk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor,
@@ -615,12 +622,13 @@ def decode_attention_blk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                          scratch: torch.Tensor | None = None) -> torch.Tensor:
     """``decode_attention`` over the block-scaled e4m3 cache that ``rope_append_blk`` writes (``kv_scales`` uint8
     [NB, PBLK / 16, HKV, 2]), with ``window`` and ``sinks`` as in ``decode_attention_window``."""
-    _fp8_cache_check(k_cache, "k_cache")
-    _fp8_cache_check(v_cache, "v_cache")
-    lead, geometry = _visible_checks(q, k_cache, v_cache, out, query_start_loc, seq_lens, block_table, window, sinks)
-    _kv_scales_check(kv_scales, k_cache)
-    return _decode_visible("fp8kv_decode_attn_blk", q, out, lead, (kv_scales.data_ptr(),), sm_scale, geometry, seq_lens,
-                           window, sinks, num_splits, max_seq_len, scratch, False)
+    dev, _, lead, geometry, NB = _attention_args(q, k_cache, v_cache, out, query_start_loc, seq_lens, block_table, window,
+                                                 sinks, False)
+    scales = _kv_scales(kv_scales, NB, geometry[4], geometry[2], dev)
+    if geometry[0] > 0:
+        _decode_visible("fp8kv_decode_attn_blk", dev, lead, (scales,), sm_scale, geometry, q, seq_lens, window, sinks,
+                        num_splits, max_seq_len, scratch, False)
+    return out
 
 
 def prefill_attention_blk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor,
@@ -629,12 +637,15 @@ def prefill_attention_blk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
                           max_query_len: int | None = None) -> torch.Tensor:
     """``prefill_attention_varlen`` over the block-scaled e4m3 cache that ``rope_append_blk`` writes, with ``window``
     and ``sinks`` as in ``prefill_attention_window``."""
-    _fp8_cache_check(k_cache, "k_cache")
-    _fp8_cache_check(v_cache, "v_cache")
-    lead, geometry = _visible_checks(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, window, sinks)
-    _kv_scales_check(kv_scales, k_cache)
-    return _prefill_visible("fp8kv_prefill_attn_blk", q, out, lead, (kv_scales.data_ptr(),), sm_scale, geometry,
-                            cu_seqlens_q, window, sinks, max_query_len)
+    dev, _, lead, geometry, NB = _attention_args(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, window,
+                                                 sinks, False)
+    scales = _kv_scales(kv_scales, NB, geometry[4], geometry[2], dev)
+    if geometry[0] == 0 or q.shape[0] == 0:
+        return out
+    if max_query_len is None:
+        max_query_len = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item())
+    _launch("fp8kv_prefill_attn_blk", dev, *lead, scales, sm_scale, *geometry, window, sinks, max_query_len)
+    return out
 
 
 # ------------------------------------------------------------------------------ layer epilogues
