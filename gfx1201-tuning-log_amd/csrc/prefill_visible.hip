@@ -17,14 +17,13 @@
 //     the first query's window on.  A 16-key group inside them that holds none is not read (nor its
 //     block-table entry): its rows are copied from the window's first group and masked.
 //   * masks are applied only on tiles that some row of the block does not see whole.
-//   * e4m3 V enters P.V in fp16, where codes are exact, and so do the weights: they keep 11 bits instead of bf16's 8
-//     and are at most 2^kRescaleSlack.  bf16 V stays bf16, and so do its weights; their sum is then taken of
-//     the rounded values, so that the weights add up to one.
 //   * block scales (SC) are powers of two.  K's byte is the A scale of the block-scaled MFMA that forms the scores
-//     anyway.  V's multiplies the weights, whose products with it are kept in range row by row: the accumulators
-//     of a row are in units of 2^e (e_run), where e + m follows the row's running maximum of log2 w + ev
-//     like m follows that of log2 w, so a row's precision goes by the keys that it sees and weighs, not by its
-//     neighbours' scales.  A group's pair of bytes is loaded with the window's copies and passed through LDS.
+//     anyway, V's the scale operand of the conversion that widens its codes to bf16, where they stay exact; neither
+//     costs an instruction per element.  A group's pair of bytes is loaded with the window's copies and passed
+//     through LDS.
+//   * the weights are rounded to bf16 for P.V, which has the range for any score and any block scale, and the sum
+//     that divides the result is that of the ROUNDED weights, so that they add up to one: a row of ones of the A operand
+//     (one MFMA per row-set) forms it, where adding up on the vector units takes 15 instructions.
 //   * a masked key's V must not reach a row through 0 * NaN: on masked tiles that hold a non-finite V
 //     (one test of the raw words), it is zeroed for the product and added afterwards to the rows that see it.
 #include "fp8kv_common.h"
@@ -40,14 +39,6 @@ struct VisibleParams : Params {
     int window, sinks;
 };
 
-typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ f32x4_t mfma16x16x32_f16(u32x4_t a, u32x4_t b, f32x4_t c)
-{
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
-}
-
 // Scores of one 16-key group: K codes times the group's scale (byte KG * 2 of `scales`) against a split
 // query row.
 template <int KG, bool LO>
@@ -55,15 +46,6 @@ __device__ __forceinline__ f32x4_t score_mfma(const v8i& k, const v8i& q, f32x4_
 {
     constexpr int qs = 127 | (127 + kQLoExp) << 8;
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q, c, 0, 0, 2 * KG, (int)scales, LO ? 1 : 0, qs);
-}
-
-__device__ __forceinline__ uint32_t f16x2_bits(f16x2_t v) { return __builtin_bit_cast(uint32_t, v); }
-__device__ __forceinline__ uint32_t pack_f16x2(float a, float b)
-{
-    f16x2_t v;
-    v[0] = (_Float16)a;
-    v[1] = (_Float16)b;
-    return f16x2_bits(v);
 }
 
 // Any non-finite element among the e4m3 codes (bf16 values) of a word.
@@ -81,43 +63,32 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w)
     return w & ~mask;
 }
 
-// rescale_rows for block-scaled V: ev[g] is the exponent of group g's scale, e_run the row's unit of o in log2.
+// Lazy rescale of RS row-sets for one tile of raw scores, as rescale_rows, with the sums of weights in the form that
+// their MFMA accumulates.
 template <int RS>
-__device__ __forceinline__ void rescale_rows_scaled(f32x4_t (&sc)[RS][2], float (&m_run)[RS], float (&l_run)[RS],
-                                                    f32x4_t (&o)[RS][8], const float (&qkr)[RS], float (&e_run)[RS],
-                                                    const float (&ev)[2])
+__device__ __forceinline__ void rescale_sums(f32x4_t (&sc)[RS][2], float (&m_run)[RS], f32x4_t (&l_run)[RS],
+                                             f32x4_t (&o)[RS][8], const float (&qkr)[RS])
 {
-    auto group_max = [&](int j, int g) {
-        return max_raw(max3_raw(sc[j][g][0], sc[j][g][1], sc[j][g][2]), sc[j][g][3]);
+    auto tile_max = [&](int j) {
+        float m = max3_raw(sc[j][0][0], sc[j][0][1], sc[j][0][2]);
+        m = max3_raw(m, sc[j][0][3], sc[j][1][0]);
+        m = max3_raw(m, sc[j][1][1], sc[j][1][2]);
+        return max_raw(m, sc[j][1][3]);
     };
-    bool any_need = false;
+    float over = kMaxFloor;                            // largest excess over a row's reference
+#pragma unroll
+    for (int j = 0; j < RS; ++j) over = max_raw(over, tile_max(j) * qkr[j] - m_run[j]);
+    if (!__any(over > kRescaleSlack)) return;
 #pragma unroll
     for (int j = 0; j < RS; ++j) {
+        asm volatile("" : "+v"(sc[j][0][0]));          // opaque: the max is formed again instead of being held over the test
+        const float mc = max_xor16_32_raw(tile_max(j)) * qkr[j];   // -inf for a fully masked row
+        const float m_new = mc > m_run[j] + kRescaleSlack ? mc : m_run[j];
+        const float alpha = __builtin_amdgcn_exp2f(m_run[j] - m_new);
+        l_run[j] *= alpha;
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            const float x = group_max(j, g) * qkr[j] - m_run[j];
-            any_need |= x > kRescaleSlack || x + ev[g] > e_run[j] + kRescaleSlack;
-        }
-    }
-    if (__any(any_need)) {
-#pragma unroll
-        for (int j = 0; j < RS; ++j) {
-            // opaque: the maxima are formed again instead of being held over the test
-            asm volatile("" : "+v"(sc[j][0][0]), "+v"(sc[j][1][0]));
-            const float m0 = max_xor16_32_raw(group_max(j, 0)) * qkr[j], m1 = max_xor16_32_raw(group_max(j, 1)) * qkr[j];
-            const float mc = max_raw(m0, m1);                      // -inf for a fully masked row
-            const float m_new = mc > m_run[j] + kRescaleSlack ? mc : m_run[j];
-            const float down = m_run[j] - m_new;
-            const float top = max_raw((m0 - m_new) + ev[0], (m1 - m_new) + ev[1]);
-            const bool need = down < 0.f || top > e_run[j] + kRescaleSlack;
-            const float e_new = need ? max_raw(e_run[j] + down, top) : e_run[j];
-            const float alpha = __builtin_amdgcn_exp2f(down + (e_run[j] - e_new));
-            l_run[j] *= __builtin_amdgcn_exp2f(down);
-#pragma unroll
-            for (int n = 0; n < 8; ++n) o[j][n] *= alpha;
-            m_run[j] = m_new;
-            e_run[j] = e_new;
-        }
+        for (int n = 0; n < 8; ++n) o[j][n] *= alpha;
+        m_run[j] = m_new;
     }
 }
 
@@ -130,7 +101,6 @@ prefill_visible_kernel(VisibleParams P)
     constexpr int TILE = B16 ? kTileBytes16 : kTileBytes;
     constexpr int NR = W / NG;
     constexpr int NT = NR * TPW;                           // tiles per window
-    constexpr bool HALVES = SC && RS > 2;                  // V widened in two halves: no registers for both at once
     static_assert(NG * NR == W && RS >= 1 && NT <= 64, "split shape");
     constexpr int kWinBytes = NT * TILE;
     constexpr int kRingBytes = 2 * kWinBytes;
@@ -201,6 +171,11 @@ prefill_visible_kernel(VisibleParams P)
     const uint32_t voff_lane = (uint32_t)dma_r * dma_s1 + dma_chunk;
     const uint8_t* const dma_base_v = P.v + (int64_t)kh * P.sv2;   // bf16: the second copy
     const uint32_t voff_lane_v = (uint32_t)dma_r * (uint32_t)P.sv1 + dma_chunk;
+
+    // Byte offsets in an e4m3 tile of this lane's fragments: K row lr, chunk lp (k_slot; chunk 4 + lp lies 64 away), and
+    // V row 4 lp, d = 8 lr (v_slot; row 4 lp + j lies 256 j behind, 16 rows further 2048).
+    const int k_lane = 1024 * (lr >> 3) + 16 * k_slot(lr & 7, lp);
+    const int v_lane = TILE / 2 + 1024 * (lp >> 1) + 16 * v_slot(4 * (lp & 1), lr >> 1) + 8 * (lr & 1);
 
     // head, and block within the workgroup, of row-set rset (those past the last repeat it)
     auto head_of = [&](int rset) {
@@ -356,16 +331,16 @@ prefill_visible_kernel(VisibleParams P)
             }
         }
 
-        float m_run[RS], l_run[RS];
-        f32x4_t o[RS][8];
+        float m_run[RS];
+        f32x4_t l_run[RS], o[RS][8];                   // l_run: the sum in every element
 #pragma unroll
         for (int j = 0; j < RS; ++j) {
             m_run[j] = kMaxFloor;
-            l_run[j] = 0.f;
+            l_run[j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int n = 0; n < 8; ++n) o[j][n] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
         }
-        [[maybe_unused]] float e_run[RS] = {};
+        const u32x4_t ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
 
         for (int i = 0; i < nwin; ++i) {
             // Everything this wave has in flight: window i's copies and scales, the block ids of window i + 1.  The
@@ -428,53 +403,32 @@ prefill_visible_kernel(VisibleParams P)
                         }
                     }
                 }
-                [[maybe_unused]] u32x4_t vf[HALVES ? 4 : 8];
-                [[maybe_unused]] uint32_t vhalf[8];
-                [[maybe_unused]] float ev[2];
-                // fp16 V^T fragments 4 w .. 4 w + 3 (d = 8c + 4w ..) from word w of the eight rows
-                auto widen_words = [&](const uint32_t (&r)[8], int w) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t x = __builtin_amdgcn_perm(r[2 * k + 1], r[2 * k], 0x05010400u);   // a0 b0 a1 b1
-                        const uint32_t y = __builtin_amdgcn_perm(r[2 * k + 1], r[2 * k], 0x07030602u);   // a2 b2 a3 b3
-                        const int at = HALVES ? 0 : 4 * w;
-                        vf[at + 0][k] = f16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x, 1.0f, false));
-                        vf[at + 1][k] = f16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x, 1.0f, true));
-                        vf[at + 2][k] = f16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)y, 1.0f, false));
-                        vf[at + 3][k] = f16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)y, 1.0f, true));
-                    }
-                };
-                auto widen = [&](const u32x2_t (&vr)[8], int w) {
-                    const uint32_t r[8] = {vr[0][w], vr[1][w], vr[2][w], vr[3][w], vr[4][w], vr[5][w], vr[6][w], vr[7][w]};
-                    widen_words(r, w);
-                };
+                [[maybe_unused]] u32x4_t vf[8];
                 if constexpr (!B16) {
                     v8i kf[2];
 #pragma unroll
                     for (int kg = 0; kg < 2; ++kg) {
-                        const int row = 16 * kg + lr;
-                        const unsigned char* kb = buf + (row >> 3) * 1024;
-                        const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(kb + 16 * k_slot(row & 7, lp));
-                        const u32x4_t hi = *reinterpret_cast<const u32x4_t*>(kb + 16 * k_slot(row & 7, 4 + lp));
+                        const u32x4_t lo = *reinterpret_cast<const u32x4_t*>(buf + k_lane + 2048 * kg);
+                        const u32x4_t hi = *reinterpret_cast<const u32x4_t*>(buf + (k_lane ^ 64) + 2048 * kg);
                         kf[kg] = (v8i){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3],
                                        (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
                     }
                     uint32_t scales = 127 | 127 << 16;
+                    float vsc[2] = {1.f, 1.f};
                     if constexpr (SC) {
                         scales = *reinterpret_cast<const uint32_t*>(lds_scales[i & 1][tw]);
-                        ev[0] = uniform((float)((int)((scales >> 8) & 255u) - 127));
-                        ev[1] = uniform((float)((int)(scales >> 24) - 127));
+                        vsc[0] = e8m0_to_f32((scales >> 8) & 255u);
+                        vsc[1] = e8m0_to_f32(scales >> 24);
                     }
                     // V^T raw rows (lane (c, p) transposes d = 8c .. 8c+7) and their widening go ahead of S^T = K.Q^T
                     u32x2_t vr[8];
 #pragma unroll
                     for (int jj = 0; jj < 8; ++jj) {
-                        const int row = (jj < 4 ? 0 : 16) + 4 * lp + (jj & 3);
-                        const unsigned char* vb = buf + 4096 + (row >> 3) * 1024;
-                        vr[jj] = *reinterpret_cast<const u32x2_t*>(vb + 16 * v_slot(row & 7, lr >> 1) + 8 * (lr & 1));
+                        vr[jj] = *reinterpret_cast<const u32x2_t*>(buf + v_lane + 256 * (jj & 3) + (jj < 4 ? 0 : 2048));
                     }
                     if (masked) {
                         uint32_t bad = 0;
+                        asm volatile("" : "+v"(bad));  // a branch: nothing of the test runs on other tiles
 #pragma unroll
                         for (int jj = 0; jj < 8; ++jj) bad |= non_finite<false>(vr[jj][0]) | non_finite<false>(vr[jj][1]);
                         poisoned = __any(bad != 0);
@@ -486,10 +440,7 @@ prefill_visible_kernel(VisibleParams P)
                             }
                         }
                     }
-                    if constexpr (!HALVES) {
-                        widen(vr, 0);
-                        widen(vr, 1);
-                    }
+                    v_fragments(vr, vf, vsc[0], vsc[1]);
 #pragma unroll
                     for (int j = 0; j < RS; ++j) {
                         const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
@@ -498,20 +449,11 @@ prefill_visible_kernel(VisibleParams P)
                         acc = score_mfma<1, false>(kf[1], qhi[j], zero, scales);
                         sc[j][1] = score_mfma<1, true>(kf[1], qlo[j], acc, scales);
                     }
-                    if constexpr (HALVES) {
+                    // Interleave: one MFMA, then up to four VALU (the V widening, 48 instructions).
 #pragma unroll
-                        for (int jj = 0; jj < 8; ++jj) {
-                            asm volatile("" : "+v"(vr[jj][0]), "+v"(vr[jj][1]));
-                            vhalf[jj] = vr[jj][1];
-                        }
-                        widen(vr, 0);
-                    } else {
-                        // Interleave: one MFMA, then up to four VALU (the V widening, 48 instructions).
-#pragma unroll
-                        for (int g = 0; g < 4 * RS; ++g) {
-                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                            __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
-                        }
+                    for (int g = 0; g < 4 * RS; ++g) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
                     }
                 }
                 if (masked) {
@@ -525,73 +467,43 @@ prefill_visible_kernel(VisibleParams P)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const int key = k0 + 16 * kg + 4 * (lm >> 4) + e;
-                                if (key > qpos || (key <= qpos - window && key >= sinks)) sc[j][kg][e] = neg_inf();
+                                const bool hidden = (key > qpos) | ((key <= qpos - window) & (key >= sinks));
+                                sc[j][kg][e] = hidden ? neg_inf() : sc[j][kg][e];
                             }
                     }
                 }
-                // Weights of row-set j in the type of P.V (the P^T operand), their sum added to l.  The product is rounded
-                // like the row max, so the largest weight is at most 2^kRescaleSlack at any score.
-                auto row_probs = [&](int j) -> u32x4_t {
-#pragma clang fp contract(off)
-                    const float nm = -m_run[j];
-                    float p[2][4];
-#pragma unroll
-                    for (int kg = 0; kg < 2; ++kg)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) p[kg][e] = __builtin_amdgcn_exp2f(sc[j][kg][e] * qkr[j] + nm);
-                    [[maybe_unused]] float f[2];
-                    if constexpr (SC) {                // a group whose keys are all masked may lie far above the row's unit
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) f[g] = __builtin_amdgcn_exp2f(fminf(ev[g] - e_run[j], 120.f));
-                    }
+                rescale_sums<RS>(sc, m_run, l_run, o, qkr);
+                // Weights of row-set j in bf16 (the P^T operand).  The max is a rounded product and the fused difference is
+                // not, so where scores are past 10^7 the largest weight is not 1 but 2^+-(half a unit in the max's last
+                // place): nothing to bf16 and its fp32 sums.
+                auto row_weights = [&](int j) -> u32x4_t {
                     u32x4_t pb;
 #pragma unroll
                     for (int d = 0; d < 4; ++d) {
-                        float& a = p[d >> 1][2 * (d & 1)];
-                        float& b = p[d >> 1][2 * (d & 1) + 1];
-                        if constexpr (SC) pb[d] = pack_f16x2(a * f[d >> 1], b * f[d >> 1]);
-                        else pb[d] = B16 ? pack_bf16x2(a, b) : pack_f16x2(a, b);
-                        if (B16) {
-                            a = __uint_as_float(pb[d] << 16);
-                            b = __uint_as_float(pb[d] & 0xFFFF0000u);
-                        }
+                        const f32x4_t& x = sc[j][d >> 1];
+                        pb[d] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (d & 1)], qkr[j], -m_run[j])),
+                                            __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (d & 1) + 1], qkr[j], -m_run[j])));
                     }
-                    l_run[j] += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
                     return pb;
                 };
+                auto add_weights = [&](int j, const u32x4_t& pb) {
+                    l_run[j] = mfma16x16x32_bf16(as_bf16x8(ones), as_bf16x8(pb), l_run[j]);
+                };
                 if constexpr (!B16) {
-                    if constexpr (SC) rescale_rows_scaled<RS>(sc, m_run, l_run, o, qkr, e_run, ev);
-                    else rescale_rows<RS>(sc, m_run, l_run, o, qkr);
-                    if constexpr (HALVES) {
-                        u32x4_t pb[RS];
 #pragma unroll
-                        for (int j = 0; j < RS; ++j) {
-                            pb[j] = row_probs(j);
+                    for (int j = 0; j < RS; ++j) {
+                        const u32x4_t pb = row_weights(j);
 #pragma unroll
-                            for (int n = 0; n < 4; ++n) o[j][n] = mfma16x16x32_f16(vf[n], pb[j], o[j][n]);
-                        }
-                        widen_words(vhalf, 1);
-#pragma unroll
-                        for (int n = 0; n < 4; ++n)
-#pragma unroll
-                            for (int j = 0; j < RS; ++j) o[j][4 + n] = mfma16x16x32_f16(vf[n], pb[j], o[j][4 + n]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < RS; ++j) {
-                            const u32x4_t pb = row_probs(j);
-#pragma unroll
-                            for (int n = 0; n < 8; ++n) o[j][n] = mfma16x16x32_f16(vf[n], pb, o[j][n]);
-                        }
+                        for (int n = 0; n < 8; ++n) o[j][n] = mfma16x16x32_bf16(as_bf16x8(vf[n]), as_bf16x8(pb), o[j][n]);
+                        add_weights(j, pb);
                     }
-                    // Interleave: the first row-set's exponentials alone, then each P.V MFMA with about three
+                    // Interleave: the first row-set's exponentials alone, then each P.V MFMA with about two
                     // VALU instructions of the next row-set's softmax.
-                    if constexpr (!HALVES) {
-                        __builtin_amdgcn_sched_group_barrier(0x002, 28, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 20, 0);
 #pragma unroll
-                        for (int g = 0; g < 8 * (RS - 1); ++g) {
-                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                            __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
-                        }
+                    for (int g = 0; g < 9 * (RS - 1); ++g) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
                     }
                 } else {
                     // Half of a V row's 16 bytes at a time: half h is d = 8c + 4h .. + 3.
@@ -611,10 +523,12 @@ prefill_visible_kernel(VisibleParams P)
                         }
                     };
                     read_half(0);
-                    rescale_rows<RS>(sc, m_run, l_run, o, qkr);
                     u32x4_t pb[RS];
 #pragma unroll
-                    for (int j = 0; j < RS; ++j) pb[j] = row_probs(j);
+                    for (int j = 0; j < RS; ++j) {
+                        pb[j] = row_weights(j);
+                        add_weights(j, pb[j]);
+                    }
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         u32x4_t va[4];
@@ -691,10 +605,9 @@ prefill_visible_kernel(VisibleParams P)
 #pragma unroll
                 for (int r = 0; r < NR; ++r) mg = fmaxf(mg, stage_m[((grp * NR + r) * RS + j) * 16 + er]);
                 const float f = __builtin_amdgcn_exp2f(m_run[j] - mg);
-                const float fo = SC ? __builtin_amdgcn_exp2f((m_run[j] - mg) + e_run[j]) : f;
-                l_run[j] *= f;
+                l_run[j][0] *= f;
 #pragma unroll
-                for (int n = 0; n < 8; ++n) o[j][n] *= fo;
+                for (int n = 0; n < 8; ++n) o[j][n] *= f;
             }
             // Row-set j is summed and written by residue j % NR, in the order of the residues behind it.
 #pragma unroll
@@ -704,7 +617,7 @@ prefill_visible_kernel(VisibleParams P)
                 float* s = stage + (((grp * RS + j) * (NR - 1)) + slot) * kStageFloats;
 #pragma unroll
                 for (int n = 0; n < 8; ++n) *reinterpret_cast<f32x4_t*>(s + (n * 64 + ln) * 4) = o[j][n];
-                s[8 * 64 * 4 + ln] = l_run[j];
+                s[8 * 64 * 4 + ln] = l_run[j][0];
             }
             lds_barrier();
 #pragma unroll
@@ -715,19 +628,18 @@ prefill_visible_kernel(VisibleParams P)
                     const float* s = stage + ((grp * RS + j) * (NR - 1) + r) * kStageFloats;
 #pragma unroll
                     for (int n = 0; n < 8; ++n) o[j][n] += *reinterpret_cast<const f32x4_t*>(s + (n * 64 + ln) * 4);
-                    l_run[j] += s[8 * 64 * 4 + ln];
+                    l_run[j][0] += s[8 * 64 * 4 + ln];
                 }
             }
         }
 #pragma unroll
         for (int j = 0; j < RS; ++j) {
             if (res != j % NR) continue;
-            const float l = sum_xor16_32(l_run[j]);
+            const float l = l_run[j][0];
             const int tok = tok0 + 16 * block_of(grp * RS + j) + er;
             if (tok >= qlen || grp * RS + j >= nbt * P.gqa) continue;
             // a row that sees no key has l = 0 and is written as zeros; NaN in l reaches the output
-            float f = l == 0.f ? 0.f : vs / l;
-            if constexpr (SC && NR == 1) f *= __builtin_amdgcn_exp2f(e_run[j]);
+            const float f = l == 0.f ? 0.f : vs / l;
             __bf16* orow = P.out + (int64_t)(q_begin + tok) * P.o_stride +
                            (int64_t)(kh * P.gqa + head_of(grp * RS + j)) * kD + 32 * ep;
 #pragma unroll

@@ -295,8 +295,8 @@ int fp8kv_prefill_attn_varlen_bf16(const void* q, int64_t q_row_stride,
  *   - Rows that see nothing are zeros: seq_lens[s] <= 0, and rows of negative position (seq_lens[s] < qlen_s).
  *   - Keys that a row does not see do not reach it, whatever they hold (a NaN or an infinity included); a
  *     non-finite element of a key that it sees reaches that element of its output.
- * The probabilities enter P.V in more than bf16's precision (decode: bf16 hi + lo parts; prefill: fp16 over e4m3
- * caches); prefill over bf16 caches rounds them to bf16 and sums the rounded values.
+ * Decode weighs V in two bf16 parts (error 2^-17 of a weight); prefill rounds the weights to bf16 and divides by
+ * the sum of the rounded ones.
  * No counterpart in the reference, whose hook leaves such layers to stock vLLM (vllm-fp8kv/fp8kv_override.py:50-64). */
 int fp8kv_decode_attn_window(const void* q, int64_t q_row_stride,
                              const void* k_cache, const void* v_cache,

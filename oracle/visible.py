@@ -29,13 +29,11 @@ def visible(p: int, length: int, window: int, sinks: int) -> torch.Tensor:
 
 
 def attention(q, k_cache, v_cache, starts, seq_lens, table, k_scale, v_scale, sm_scale, window=0, sinks=0):
-    """(out [T, HQ, D], sum_t w_t |V_t| of the same shape, largest sm_scale * sum_d |q_d K_td| per row [T, HQ],
-    sum_t |V_t| / s_t times the row's largest w_t s_t, s_t the scale of V_t: what an absolute error of 1 in every weight,
-    in units of the largest weight times scale, would make)."""
+    """(out [T, HQ, D], sum_t w_t |V_t| of the same shape, largest sm_scale * sum_d |q_d K_td| per row [T, HQ])."""
     T, HQ, D = q.shape
     HKV = k_cache.shape[2]
     out = torch.zeros(T, HQ, D, dtype=torch.float64)
-    mass, floor, reach = torch.zeros_like(out), torch.zeros_like(out), torch.zeros(T, HQ, dtype=torch.float64)
+    mass, reach = torch.zeros_like(out), torch.zeros(T, HQ, dtype=torch.float64)
     for s in range(table.shape[0]):
         a, b, length = int(starts[s]), int(starts[s + 1]), int(seq_lens[s])
         for row in range(a, b):
@@ -51,10 +49,5 @@ def attention(q, k_cache, v_cache, starts, seq_lens, table, k_scale, v_scale, sm
                 w = torch.softmax(x @ k.T * sm_scale, -1)
                 out[row, heads] = w @ v
                 mass[row, heads] = w @ v.abs()
-                unit = torch.ones(pos.numel(), dtype=torch.float64)
-                if isinstance(v_scale, tuple):
-                    blk, slot = table[s].long()[pos // v_cache.shape[1]], pos % v_cache.shape[1]
-                    unit = torch.exp2(v_scale[0][blk, slot // 16, h, v_scale[1]].double() - 127)
-                floor[row, heads] = (w * unit).amax(-1, keepdim=True) * (v.abs() / unit[:, None]).sum(0)
                 reach[row, heads] = (x.abs() @ k.abs().T).amax(-1) * abs(sm_scale)
-    return out, mass, reach, floor
+    return out, mass, reach

@@ -1,11 +1,8 @@
 """GPU parity of windowed attention and of attention over block-scaled caches against the 64-bit oracle.
 
 Bound of an output element o = sum w v: its bf16 rounding, 2^-8 |o|, and on the weights, times sum w |v|:
-  * their rounding in P.V: 2^-16 (decode, two bf16 parts of 8 bits each), 2^-11 (prefill, fp16 over e4m3), or 2^-8
-    (prefill over bf16 caches);
-  * prefill over e4m3 holds a weight times its V scale in fp16, in units that the row's largest such product reaches:
-    below 2^-14 of the unit fp16 has steps of 2^-24, so the weight is off by up to 2^-25 units whatever its size, and
-    the element by 2^-25 * max(w s) * sum |v| / s over the keys that the row sees;
+  * their rounding in P.V: 2^-16 (decode, two bf16 parts of 8 bits each) or twice 2^-8 (prefill: bf16, the weight
+    and, as the sum is that of the rounded weights, the sum);
   * the scores' fp32 error: 128 products and the k-parts' sums, at most 140 * 2^-24 of sum |q k|, twice (weight and
     sum of weights), the split query's 2^-22 included, and exp2 and the running sums, some 2^-20.
 Every slot that no query sees holds NaN, and block-table entries of blocks that none needs point to a block of NaN.
@@ -22,7 +19,7 @@ from oracle import rope_append, visible
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda")
 D = 128
-PARTS = {"decode": 2.0 ** -16, "prefill": 2.0 ** -11, "prefill_bf16": 2.0 ** -8}
+PARTS = {"decode": 2.0 ** -16, "prefill": 2.0 ** -7}
 
 
 def _case(kind, lens, HQ, HKV, PBLK, window, sinks, seed=0, spread=1.0):
@@ -93,10 +90,8 @@ def _oracle(c):
     return visible.attention(c["q"], k, v, c["starts"], c["seq_lens"], c["table"], ks, vs, c["sm"], c["window"], c["sinks"])
 
 
-def _tolerance(c, form, want, mass, reach, floor):
-    part = PARTS["prefill_bf16" if form == "prefill" and c["kind"] == "bf16" else form]
-    half = 2.0 ** -25 if form == "prefill" and c["kind"] != "bf16" else 0.0
-    return 2.0 ** -8 * want.abs() + (part + 280 * 2.0 ** -24 * reach[..., None] + 2.0 ** -20) * mass + half * floor + 1e-30
+def _tolerance(c, form, want, mass, reach):
+    return 2.0 ** -8 * want.abs() + (PARTS[form] + 280 * 2.0 ** -24 * reach[..., None] + 2.0 ** -20) * mass + 1e-30
 
 
 def _check(c, form, **more):
