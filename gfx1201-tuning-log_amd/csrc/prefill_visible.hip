@@ -22,8 +22,8 @@
 //     costs an instruction per element.  A group's pair of bytes is loaded with the window's copies and passed
 //     through LDS.
 //   * the weights are rounded to bf16 for P.V, which has the range for any score and any block scale, and the sum
-//     that divides the result is that of the ROUNDED weights, so that they add up to one: a row of ones of the A operand
-//     (one MFMA per row-set) forms it, where adding up on the vector units takes 15 instructions.
+//     that divides the result is that of the ROUNDED weights, so that they add up to one (v_dot2_f32_bf16 with ones:
+//     four instructions for a row-set's eight weights).
 //   * a masked key's V must not reach a row through 0 * NaN: on masked tiles that hold a non-finite V
 //     (one test of the raw words), it is zeroed for the product and added afterwards to the rows that see it.
 #include "fp8kv_common.h"
@@ -63,33 +63,10 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w)
     return w & ~mask;
 }
 
-// Lazy rescale of RS row-sets for one tile of raw scores, as rescale_rows, with the sums of weights in the form that
-// their MFMA accumulates.
-template <int RS>
-__device__ __forceinline__ void rescale_sums(f32x4_t (&sc)[RS][2], float (&m_run)[RS], f32x4_t (&l_run)[RS],
-                                             f32x4_t (&o)[RS][8], const float (&qkr)[RS])
+// l plus the two bf16 values of w.
+__device__ __forceinline__ float add_bf16x2(uint32_t w, float l)
 {
-    auto tile_max = [&](int j) {
-        float m = max3_raw(sc[j][0][0], sc[j][0][1], sc[j][0][2]);
-        m = max3_raw(m, sc[j][0][3], sc[j][1][0]);
-        m = max3_raw(m, sc[j][1][1], sc[j][1][2]);
-        return max_raw(m, sc[j][1][3]);
-    };
-    float over = kMaxFloor;                            // largest excess over a row's reference
-#pragma unroll
-    for (int j = 0; j < RS; ++j) over = max_raw(over, tile_max(j) * qkr[j] - m_run[j]);
-    if (!__any(over > kRescaleSlack)) return;
-#pragma unroll
-    for (int j = 0; j < RS; ++j) {
-        asm volatile("" : "+v"(sc[j][0][0]));          // opaque: the max is formed again instead of being held over the test
-        const float mc = max_xor16_32_raw(tile_max(j)) * qkr[j];   // -inf for a fully masked row
-        const float m_new = mc > m_run[j] + kRescaleSlack ? mc : m_run[j];
-        const float alpha = __builtin_amdgcn_exp2f(m_run[j] - m_new);
-        l_run[j] *= alpha;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) o[j][n] *= alpha;
-        m_run[j] = m_new;
-    }
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), __builtin_bit_cast(bf16x2_t, 0x3F803F80u), l, false);
 }
 
 // SC: block-scaled e4m3 caches.
@@ -167,10 +144,9 @@ prefill_visible_kernel(VisibleParams P)
     const uint8_t* dma_base = dma_v ? P.v + (int64_t)kh * P.sv2 : P.k + (int64_t)kh * P.sk2;
     const int64_t dma_s0 = dma_v ? P.sv0 : P.sk0;
     const uint32_t dma_s1 = (uint32_t)(dma_v ? P.sv1 : P.sk1);    // < 2^32 / block size (host check)
-    const uint32_t dma_chunk = 16u * (uint32_t)dma_c;
-    const uint32_t voff_lane = (uint32_t)dma_r * dma_s1 + dma_chunk;
+    const uint32_t voff_lane = (uint32_t)dma_r * dma_s1 + 16u * (uint32_t)dma_c;
     const uint8_t* const dma_base_v = P.v + (int64_t)kh * P.sv2;   // bf16: the second copy
-    const uint32_t voff_lane_v = (uint32_t)dma_r * (uint32_t)P.sv1 + dma_chunk;
+    const uint32_t voff_lane_v = (uint32_t)dma_r * (uint32_t)P.sv1 + 16u * (uint32_t)dma_c;
 
     // Byte offsets in an e4m3 tile of this lane's fragments: K row lr, chunk lp (k_slot; chunk 4 + lp lies 64 away), and
     // V row 4 lp, d = 8 lr (v_slot; row 4 lp + j lies 256 j behind, 16 rows further 2048).
@@ -198,58 +174,50 @@ prefill_visible_kernel(VisibleParams P)
         const int nwin = (ntiles + NT - 1) / NT;
         const int first_group = low >> 4;
         auto tile_at = [&](int t) { return t + (t >= head ? jump : 0); };
-        // First key that this wave's copy of walked tile t reads: of its own group, or of the window's first
-        // where nobody sees a key of its own.
+        // First key that this wave's copy of walked tile t reads: of its own 16-key group, or, where nobody sees a key
+        // of that, of one that is there: the window's first, and behind the last key the last.  Slots of a group behind
+        // the last key are read as they are: masks and the test for non-finite V take care of what they hold.
+        const int last_group = (k_hi - 1) >> 4;
         auto copy_key = [&](int t) {
-            const int row = kBN * tile_at(t) + dma_row0;
-            const int g = row >> 4;
-            return g >= first_group || 16 * g < sinks ? row : 16 * first_group + (dma_row0 & 15);
+            int g = 2 * tile_at(t) + (dma_row0 >> 4);
+            g = (g >= first_group) | (16 * g < sinks) ? g : first_group;
+            return 16 * min(g, last_group) + (dma_row0 & 15);
         };
         auto token_of = [&](int j) { return tok0 + 16 * block_of(grp * RS + j) + lr; };
         // Several blocks: keys past this wave's last row, and below its first row's window, are left out.
         const int my_hi = MB ? qfirst + 16 * block_of(grp * RS + RS - 1) + 15 : k_hi;
         const int my_low = MB ? qfirst + 16 * block_of(grp * RS) - window + 1 : 0;
 
-        // Block ids for this wave's copy of each tile of window wi: lane u holds that of its tile u.
+        // A window's copies are prepared by lane: lane u holds the block id, then the address, of tile u's first row, and
+        // a copy takes it from there with two readlanes (formed by scalar instructions, copy by copy, addresses were
+        // most of a tile's instructions).  Scale bytes of the window's groups come along in the two waves whose K copies
+        // are those of a tile's groups (rows 0 and 16).
         int bids = 0;
-        auto load_bids = [&](int wi) {
-            const int key0 = min(copy_key(wi * NT + lane), k_hi - 1);
-            bids = lane < NT ? btrow[key0 >> P.pshift] : 0;
-        };
-        // Scale bytes of window wi's groups, by the two waves whose K copies cover a tile's groups (rows 0 and 16): lane u
-        // those of tile u.  Follows load_bids(wi).
+        uint64_t src = 0;
+        [[maybe_unused]] uint64_t src_v = 0;
         [[maybe_unused]] uint32_t sc_next = 0;
-        auto load_scales = [&](int wi) {
+        auto load_bids = [&](int wi) { bids = lane < NT ? btrow[copy_key(wi * NT + lane) >> P.pshift] : 0; };
+        auto place_window = [&](int wi) {
+            const uint32_t slot = (uint32_t)(copy_key(wi * NT + lane) & (P.pblk - 1));
+            src = (uint64_t)dma_base + (int64_t)bids * dma_s0 + (uint64_t)slot * dma_s1;
+            if constexpr (B16) src_v = (uint64_t)dma_base_v + (int64_t)bids * P.sv0 + (uint64_t)slot * (uint32_t)P.sv1;
             if constexpr (SC) {
-                if ((wave == 0 || wave == 2) && lane < NT) {
-                    const int key0 = min(copy_key(wi * NT + lane), k_hi - 1);
-                    sc_next = P.kv_scales[((int64_t)bids * (P.pblk >> 4) + ((key0 & (P.pblk - 1)) >> 4)) * P.hkv + kh];
-                }
+                if ((wave == 0 || wave == 2) && lane < NT)
+                    sc_next = P.kv_scales[((int64_t)bids * (P.pblk >> 4) + (slot >> 4)) * P.hkv + kh];
             }
         };
-        // Copies of tiles u0 .. u1 - 1 of window wi (keys >= k_hi fetch key k_hi - 1; the causal mask removes them).
+        auto lane_address = [&](uint64_t a, int u) -> const uint8_t* {
+            const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)a, u), hi = __builtin_amdgcn_readlane((uint32_t)(a >> 32), u);
+            return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
+        };
+        // Copies of tiles u0 .. u1 - 1 of window wi.
         auto issue_window = [&](int wi, int u0, int u1) {
 #pragma unroll
             for (int u = u0; u < u1; ++u) {
-                const int t = wi * NT + u;
-                if (t < ntiles) {
-                    const int64_t b = __builtin_amdgcn_readlane(bids, u);
-                    const uint8_t* sb = dma_base + b * dma_s0;
-                    const uint8_t* sbv = dma_base_v + b * P.sv0;
-                    uint32_t voff = voff_lane, voff_v = voff_lane_v;
-                    const int key = copy_key(t);
-                    if (key + 16 > k_hi) {                  // near the end of the keys
-                        const uint32_t slot = (uint32_t)(min(key + dma_r, k_hi - 1) & (P.pblk - 1));
-                        voff = slot * dma_s1 + dma_chunk;
-                        voff_v = slot * (uint32_t)P.sv1 + dma_chunk;
-                    } else {
-                        const uint32_t slot = (uint32_t)(key & (P.pblk - 1));
-                        sb += slot * dma_s1;
-                        sbv += slot * (uint32_t)P.sv1;
-                    }
+                if (wi * NT + u < ntiles) {
                     unsigned char* dst = ring + (wi & 1) * kWinBytes + u * TILE + wave * 1024;
-                    dma16_saddr(sb, voff, dst);
-                    if constexpr (B16) dma16_saddr(sbv, voff_v, dst + TILE / 2);
+                    dma16_saddr(lane_address(src, u), voff_lane, dst);
+                    if constexpr (B16) dma16_saddr(lane_address(src_v, u), voff_lane_v, dst + TILE / 2);
                 }
             }
         };
@@ -283,6 +251,7 @@ prefill_visible_kernel(VisibleParams P)
                     qlo[j][4 + d] = (int)(qf[j][3][d] ^ qflip);
                 }
             }
+            place_window(0);
             issue_window(0, 0, NT);
             if (1 < nwin) load_bids(1);
         } else {
@@ -299,8 +268,8 @@ prefill_visible_kernel(VisibleParams P)
 #pragma unroll
             for (int u = 0; u < PER; ++u)
                 asm volatile("" : "+v"(qf[u][0]), "+v"(qf[u][1]), "+v"(qf[u][2]), "+v"(qf[u][3]));
+            place_window(0);
             issue_window(0, 0, NT);
-            if (nwin > 0) load_scales(0);
             if (1 < nwin) load_bids(1);
 #pragma unroll
             for (int u = 0; u < PER; ++u) {
@@ -331,16 +300,15 @@ prefill_visible_kernel(VisibleParams P)
             }
         }
 
-        float m_run[RS];
-        f32x4_t l_run[RS], o[RS][8];                   // l_run: the sum in every element
+        float m_run[RS], l_run[RS];
+        f32x4_t o[RS][8];
 #pragma unroll
         for (int j = 0; j < RS; ++j) {
             m_run[j] = kMaxFloor;
-            l_run[j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+            l_run[j] = 0.f;
 #pragma unroll
             for (int n = 0; n < 8; ++n) o[j][n] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
         }
-        const u32x4_t ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
 
         for (int i = 0; i < nwin; ++i) {
             // Everything this wave has in flight: window i's copies and scales, the block ids of window i + 1.  The
@@ -351,14 +319,12 @@ prefill_visible_kernel(VisibleParams P)
             }
             lds_barrier();
             const bool more = i + 1 < nwin;
+            if (more) place_window(i + 1);
 
 #pragma unroll
             for (int v = 0; v < TPW; ++v) {
                 // The next window's copies go out in TPW parts, one before each tile.
-                if (more) {
-                    issue_window(i + 1, v * NT / TPW, (v + 1) * NT / TPW);
-                    if (v == 0) load_scales(i + 1);
-                }
+                if (more) issue_window(i + 1, v * NT / TPW, (v + 1) * NT / TPW);
                 const int tw = res * TPW + v;                    // tile within the window
                 const int t = i * NT + tw;
                 const int k0 = kBN * tile_at(t);
@@ -417,8 +383,9 @@ prefill_visible_kernel(VisibleParams P)
                     float vsc[2] = {1.f, 1.f};
                     if constexpr (SC) {
                         scales = *reinterpret_cast<const uint32_t*>(lds_scales[i & 1][tw]);
-                        vsc[0] = e8m0_to_f32((scales >> 8) & 255u);
-                        vsc[1] = e8m0_to_f32(scales >> 24);
+                        const uint32_t u = __builtin_amdgcn_readfirstlane(scales);
+                        vsc[0] = __uint_as_float((u & 0xFF00u) << 15);         // bytes 1 .. 254 are exponents as they are
+                        vsc[1] = __uint_as_float((u & 0xFF000000u) >> 1);
                     }
                     // V^T raw rows (lane (c, p) transposes d = 8c .. 8c+7) and their widening go ahead of S^T = K.Q^T
                     u32x2_t vr[8];
@@ -472,7 +439,7 @@ prefill_visible_kernel(VisibleParams P)
                             }
                     }
                 }
-                rescale_sums<RS>(sc, m_run, l_run, o, qkr);
+                rescale_rows<RS>(sc, m_run, l_run, o, qkr);
                 // Weights of row-set j in bf16 (the P^T operand).  The max is a rounded product and the fused difference is
                 // not, so where scores are past 10^7 the largest weight is not 1 but 2^+-(half a unit in the max's last
                 // place): nothing to bf16 and its fp32 sums.
@@ -484,10 +451,8 @@ prefill_visible_kernel(VisibleParams P)
                         pb[d] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (d & 1)], qkr[j], -m_run[j])),
                                             __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (d & 1) + 1], qkr[j], -m_run[j])));
                     }
+                    l_run[j] = add_bf16x2(pb[3], add_bf16x2(pb[2], add_bf16x2(pb[1], add_bf16x2(pb[0], l_run[j]))));
                     return pb;
-                };
-                auto add_weights = [&](int j, const u32x4_t& pb) {
-                    l_run[j] = mfma16x16x32_bf16(as_bf16x8(ones), as_bf16x8(pb), l_run[j]);
                 };
                 if constexpr (!B16) {
 #pragma unroll
@@ -495,15 +460,14 @@ prefill_visible_kernel(VisibleParams P)
                         const u32x4_t pb = row_weights(j);
 #pragma unroll
                         for (int n = 0; n < 8; ++n) o[j][n] = mfma16x16x32_bf16(as_bf16x8(vf[n]), as_bf16x8(pb), o[j][n]);
-                        add_weights(j, pb);
                     }
-                    // Interleave: the first row-set's exponentials alone, then each P.V MFMA with about two
+                    // Interleave: the first row-set's exponentials alone, then each P.V MFMA with three
                     // VALU instructions of the next row-set's softmax.
-                    __builtin_amdgcn_sched_group_barrier(0x002, 20, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 24, 0);
 #pragma unroll
-                    for (int g = 0; g < 9 * (RS - 1); ++g) {
+                    for (int g = 0; g < 8 * (RS - 1); ++g) {
                         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
                     }
                 } else {
                     // Half of a V row's 16 bytes at a time: half h is d = 8c + 4h .. + 3.
@@ -525,10 +489,7 @@ prefill_visible_kernel(VisibleParams P)
                     read_half(0);
                     u32x4_t pb[RS];
 #pragma unroll
-                    for (int j = 0; j < RS; ++j) {
-                        pb[j] = row_weights(j);
-                        add_weights(j, pb[j]);
-                    }
+                    for (int j = 0; j < RS; ++j) pb[j] = row_weights(j);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         u32x4_t va[4];
@@ -605,7 +566,7 @@ prefill_visible_kernel(VisibleParams P)
 #pragma unroll
                 for (int r = 0; r < NR; ++r) mg = fmaxf(mg, stage_m[((grp * NR + r) * RS + j) * 16 + er]);
                 const float f = __builtin_amdgcn_exp2f(m_run[j] - mg);
-                l_run[j][0] *= f;
+                l_run[j] *= f;
 #pragma unroll
                 for (int n = 0; n < 8; ++n) o[j][n] *= f;
             }
@@ -617,7 +578,7 @@ prefill_visible_kernel(VisibleParams P)
                 float* s = stage + (((grp * RS + j) * (NR - 1)) + slot) * kStageFloats;
 #pragma unroll
                 for (int n = 0; n < 8; ++n) *reinterpret_cast<f32x4_t*>(s + (n * 64 + ln) * 4) = o[j][n];
-                s[8 * 64 * 4 + ln] = l_run[j][0];
+                s[8 * 64 * 4 + ln] = l_run[j];
             }
             lds_barrier();
 #pragma unroll
@@ -628,14 +589,14 @@ prefill_visible_kernel(VisibleParams P)
                     const float* s = stage + ((grp * RS + j) * (NR - 1) + r) * kStageFloats;
 #pragma unroll
                     for (int n = 0; n < 8; ++n) o[j][n] += *reinterpret_cast<const f32x4_t*>(s + (n * 64 + ln) * 4);
-                    l_run[j][0] += s[8 * 64 * 4 + ln];
+                    l_run[j] += s[8 * 64 * 4 + ln];
                 }
             }
         }
 #pragma unroll
         for (int j = 0; j < RS; ++j) {
             if (res != j % NR) continue;
-            const float l = l_run[j][0];
+            const float l = sum_xor16_32(l_run[j]);
             const int tok = tok0 + 16 * block_of(grp * RS + j) + er;
             if (tok >= qlen || grp * RS + j >= nbt * P.gqa) continue;
             // a row that sees no key has l = 0 and is written as zeros; NaN in l reaches the output

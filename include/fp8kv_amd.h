@@ -348,7 +348,7 @@ int fp8kv_prefill_attn_window_bf16(const void* q, int64_t q_row_stride,
  * Attention over a block-scaled cache (fp8kv_rope_append_blk): e4m3 codes with one power-of-two scale per 16
  * tokens, kv head and tensor,
  *   K_t = code * 2^(b_K - 127), V_t = code * 2^(b_V - 127), b = kv_scales[block][slot / 16][kv head],
- * kv_scales uint8 [blocks, block_size / 16, num_kv_heads, 2] contiguous, 2-byte aligned, bytes below 255.  With
+ * kv_scales uint8 [blocks, block_size / 16, num_kv_heads, 2] contiguous, 2-byte aligned, bytes in [1, 254].  With
  * window and sinks as above (0, 0: whole causal contexts); everything else, the guarantees too, as there.
  * No counterpart in the reference. */
 int fp8kv_decode_attn_blk(const void* q, int64_t q_row_stride,
