@@ -117,6 +117,12 @@ int fp8kv_gemm_plan(int N, int K, int M, int token);
  * The events are used once; a rejected call leaves them armed for the next launch. */
 void fp8kv_time_next_launch(void* start_event, void* stop_event);
 
+/* Launch plan of the visible-key prefill calls (csrc/prefill_visible.hip), nothing launched: out[5] = row-sets per wave,
+ * groups of row-sets, token blocks of 16 per workgroup, whether blocks come in pairs, workgroups per (sequence, kv
+ * head) of the longest sequence.  bf16: over bf16 caches. */
+int fp8kv_prefill_visible_plan(int num_q_heads, int num_kv_heads, int num_seqs, int max_query_len, int num_tokens,
+                               int window, int sinks, int bf16, int* out);
+
 #ifdef __cplusplus
 }
 #endif

@@ -28,6 +28,7 @@
 //     (one test of the raw words), it is zeroed for the product and added afterwards to the rows that see it.
 #include "fp8kv_common.h"
 #include "fp8kv_status.h"
+#include "fp8kv_diag.h"
 #include "attn_common.h"
 #include "prefill_tiles.h"
 
@@ -70,7 +71,7 @@ __device__ __forceinline__ float add_bf16x2(uint32_t w, float l)
 }
 
 // SC: block-scaled e4m3 caches.
-template <int RS, int NG, int TPW, bool B16, bool MB, bool SC>
+template <int RS, int NG, int TPW, bool B16, bool SC>
 __global__ void __launch_bounds__(kSplitWaves * 64)
 prefill_visible_kernel(VisibleParams P)
 {
@@ -78,14 +79,16 @@ prefill_visible_kernel(VisibleParams P)
     constexpr int TILE = B16 ? kTileBytes16 : kTileBytes;
     constexpr int NR = W / NG;
     constexpr int NT = NR * TPW;                           // tiles per window
+    constexpr int UNROLL = TPW <= 2 ? TPW : 1;
     static_assert(NG * NR == W && RS >= 1 && NT <= 64, "split shape");
     constexpr int kWinBytes = NT * TILE;
     constexpr int kRingBytes = 2 * kWinBytes;
     constexpr int kStageBytes = NG * RS * (NR - 1) * kStageFloats * 4;
-    // the query rows' hand-over: the ring's second window, or behind the ring where that is too small
+    // the query rows' hand-over, from the ring's second window on: that is written only after the first barrier of the
+    // key loop
     constexpr int kSetBytes = 4 * 1024 + 256;
-    constexpr int kExch = NG * RS * kSetBytes <= kWinBytes ? kWinBytes : kRingBytes;
-    constexpr int kExchEnd = B16 ? 0 : kExch + NG * RS * kSetBytes;
+    constexpr int kExch = kWinBytes;
+    constexpr int kExchEnd = B16 || NR == 1 ? 0 : kExch + NG * RS * kSetBytes;
     constexpr int kLoopBytes = kRingBytes > kExchEnd ? kRingBytes : kExchEnd;
     __shared__ __align__(16) unsigned char ring[kLoopBytes > kStageBytes ? kLoopBytes : kStageBytes];
     __shared__ float stage_m[NR > 1 ? NG * NR * RS * 16 : 4];
@@ -113,7 +116,7 @@ prefill_visible_kernel(VisibleParams P)
 
     const int q_begin = P.cu_q[seq], qlen = P.cu_q[seq + 1] - q_begin;
     const int q0 = P.seq_lens[seq] - qlen;                         // may be negative: those rows see nothing
-    const int nbt = MB ? P.nb : 1;                                 // token blocks of 16 per workgroup
+    const int nbt = P.nb;                                          // token blocks of 16 per workgroup
     const int n16 = (qlen + 16 * nbt - 1) / (16 * nbt);
     const int tb = P.ntb_grid - 1 - rank;
     const int nwg = P.paired ? (n16 + 1) >> 1 : n16;              // workgroups this sequence needs
@@ -154,11 +157,12 @@ prefill_visible_kernel(VisibleParams P)
     const int v_lane = TILE / 2 + 1024 * (lp >> 1) + 16 * v_slot(4 * (lp & 1), lr >> 1) + 8 * (lr & 1);
 
     // head, and block within the workgroup, of row-set rset (those past the last repeat it)
-    auto head_of = [&](int rset) {
-        rset = min(rset, nbt * P.gqa - 1);
-        return MB ? rset % P.gqa : rset;
-    };
-    auto block_of = [&](int rset) { return MB ? min(rset, nbt * P.gqa - 1) / P.gqa : 0; };
+    const int last_set = nbt * P.gqa - 1;
+    auto head_of = [&](int rset) { return min(rset, last_set) % P.gqa; };
+    auto block_of = [&](int rset) { return min(rset, last_set) / P.gqa; };
+    int my_block[RS];                                              // block of this wave's row-sets
+#pragma unroll
+    for (int j = 0; j < RS; ++j) my_block[j] = block_of(grp * RS + j);
 
     for (int ph = 0; ph < nphase; ++ph) {
         const int blk = ph == 0 ? blk_b : blk_a;
@@ -183,10 +187,10 @@ prefill_visible_kernel(VisibleParams P)
             g = (g >= first_group) | (16 * g < sinks) ? g : first_group;
             return 16 * min(g, last_group) + (dma_row0 & 15);
         };
-        auto token_of = [&](int j) { return tok0 + 16 * block_of(grp * RS + j) + lr; };
-        // Several blocks: keys past this wave's last row, and below its first row's window, are left out.
-        const int my_hi = MB ? qfirst + 16 * block_of(grp * RS + RS - 1) + 15 : k_hi;
-        const int my_low = MB ? qfirst + 16 * block_of(grp * RS) - window + 1 : 0;
+        auto token_of = [&](int j) { return tok0 + 16 * my_block[j] + lr; };
+        // Tiles past this wave's last row, and below its first row's window, are left out.
+        const int my_hi = qfirst + 16 * my_block[RS - 1] + 15;
+        const int my_low = qfirst + 16 * my_block[0] - window + 1;
 
         // A window's copies are prepared by lane: lane u holds the block id, then the address, of tile u's first row, and
         // a copy takes it from there with two readlanes (formed by scalar instructions, copy by copy, addresses were
@@ -210,16 +214,23 @@ prefill_visible_kernel(VisibleParams P)
             const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)a, u), hi = __builtin_amdgcn_readlane((uint32_t)(a >> 32), u);
             return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
         };
-        // Copies of tiles u0 .. u1 - 1 of window wi.
-        auto issue_window = [&](int wi, int u0, int u1) {
+        // Copies of part v of window wi: tiles NR v .. NR v + NR - 1.
+        auto issue_part = [&](int wi, int v) {
 #pragma unroll
-            for (int u = u0; u < u1; ++u) {
+            for (int k = 0; k < NR; ++k) {
+                const int u = NR * v + k;
                 if (wi * NT + u < ntiles) {
                     unsigned char* dst = ring + (wi & 1) * kWinBytes + u * TILE + wave * 1024;
                     dma16_saddr(lane_address(src, u), voff_lane, dst);
                     if constexpr (B16) dma16_saddr(lane_address(src_v, u), voff_lane_v, dst + TILE / 2);
                 }
             }
+        };
+        auto first_window = [&]() {
+            place_window(0);
+#pragma unroll UNROLL
+            for (int v = 0; v < TPW; ++v) issue_part(0, v);
+            if (1 < nwin) load_bids(1);
         };
         // Q as the B operand of S^T = K.Q^T: see prefill_attn.hip.  e4m3 caches: hi + lo parts, split by one wave per row-set
         // and handed over through the LDS; bf16 caches: the four fragments, loaded by each wave.
@@ -251,9 +262,18 @@ prefill_visible_kernel(VisibleParams P)
                     qlo[j][4 + d] = (int)(qf[j][3][d] ^ qflip);
                 }
             }
-            place_window(0);
-            issue_window(0, 0, NT);
-            if (1 < nwin) load_bids(1);
+            first_window();
+        } else if constexpr (NR == 1) {
+            // every wave has row-sets of its own
+            u32x4_t qf[RS][4];
+#pragma unroll
+            for (int j = 0; j < RS; ++j) load_query(qf[j], token_of(j), head_of(grp * RS + j));
+#pragma unroll
+            for (int j = 0; j < RS; ++j)
+                asm volatile("" : "+v"(qf[j][0]), "+v"(qf[j][1]), "+v"(qf[j][2]), "+v"(qf[j][3]));
+            first_window();
+#pragma unroll
+            for (int j = 0; j < RS; ++j) qkr[j] = fmaxf(qk * q_fp8_split(qf[j], qflip, qhi[j], qlo[j]), kMinFactor16);
         } else {
             constexpr int SETS = NG * RS, PER = (SETS + W - 1) / W;        // row-sets, and splits per wave at most
             unsigned char* const exch = ring + kExch;
@@ -268,9 +288,7 @@ prefill_visible_kernel(VisibleParams P)
 #pragma unroll
             for (int u = 0; u < PER; ++u)
                 asm volatile("" : "+v"(qf[u][0]), "+v"(qf[u][1]), "+v"(qf[u][2]), "+v"(qf[u][3]));
-            place_window(0);
-            issue_window(0, 0, NT);
-            if (1 < nwin) load_bids(1);
+            first_window();
 #pragma unroll
             for (int u = 0; u < PER; ++u) {
                 const int rset = wave + W * u;
@@ -321,17 +339,18 @@ prefill_visible_kernel(VisibleParams P)
             const bool more = i + 1 < nwin;
             if (more) place_window(i + 1);
 
-#pragma unroll
+#pragma unroll UNROLL
             for (int v = 0; v < TPW; ++v) {
                 // The next window's copies go out in TPW parts, one before each tile.
-                if (more) issue_window(i + 1, v * NT / TPW, (v + 1) * NT / TPW);
+                if (more) issue_part(i + 1, v);
                 const int tw = res * TPW + v;                    // tile within the window
                 const int t = i * NT + tw;
                 const int k0 = kBN * tile_at(t);
-                if (t >= ntiles || (MB && (k0 > my_hi || (k0 + kBN <= my_low && k0 >= sinks)))) continue;
+                if (t >= ntiles || k0 > my_hi || (k0 + kBN <= my_low && k0 >= sinks)) continue;
                 const unsigned char* buf = ring + (i & 1) * kWinBytes + tw * TILE;
-                // Some row does not see some key: past the first query, or below the last one's window and no sink.
-                const bool masked = k0 + kBN - 1 > qfirst || (k0 <= qlast - window && k0 + kBN > sinks);
+                // Some row of this wave does not see some key: past its first query, or below its last one's window and no sink.
+                const bool masked = k0 + kBN - 1 > qfirst + 16 * my_block[0] ||
+                                    (k0 <= min(qlast, my_hi) - window && k0 + kBN > sinks);
                 f32x4_t sc[RS][2];
                 bool poisoned = false;
                 if constexpr (B16) {
@@ -428,7 +447,7 @@ prefill_visible_kernel(VisibleParams P)
                     asm volatile("" : "+v"(lm));
 #pragma unroll
                     for (int j = 0; j < RS; ++j) {
-                        const int qpos = q0 + tok0 + 16 * block_of(grp * RS + j) + (lm & 15);
+                        const int qpos = q0 + tok0 + 16 * my_block[j] + (lm & 15);
 #pragma unroll
                         for (int kg = 0; kg < 2; ++kg)
 #pragma unroll
@@ -526,7 +545,7 @@ prefill_visible_kernel(VisibleParams P)
                                 if (!__any(non_finite<B16>(w) != 0)) continue;
 #pragma unroll
                                 for (int j = 0; j < RS; ++j) {
-                                    const int qpos = q0 + tok0 + 16 * block_of(grp * RS + j) + (ln & 15);
+                                    const int qpos = q0 + tok0 + 16 * my_block[j] + (ln & 15);
                                     const bool sees = key <= qpos && (key > qpos - window || key < sinks);
                                     constexpr int per = B16 ? 2 : 4;               // elements of a word
 #pragma unroll
@@ -597,7 +616,7 @@ prefill_visible_kernel(VisibleParams P)
         for (int j = 0; j < RS; ++j) {
             if (res != j % NR) continue;
             const float l = sum_xor16_32(l_run[j]);
-            const int tok = tok0 + 16 * block_of(grp * RS + j) + er;
+            const int tok = tok0 + 16 * my_block[j] + er;
             if (tok >= qlen || grp * RS + j >= nbt * P.gqa) continue;
             // a row that sees no key has l = 0 and is written as zeros; NaN in l reaches the output
             const float f = l == 0.f ? 0.f : vs / l;
@@ -619,44 +638,89 @@ prefill_visible_kernel(VisibleParams P)
     }
 }
 
-template <bool SC>
-void launch_e4m3(const VisibleParams& P, dim3 grid, dim3 block, hipStream_t stream)
+// ---- launch plan ----------------------------------------------------------------------------------
+// A workgroup takes nb token blocks of 16, whose nb * GQA row-sets fill the smallest shape that holds them.  More
+// blocks share the copies of their keys (which run at the L2's rate for one block of GQA 4 over bf16 caches), start and
+// end once, and leave fewer partial states to merge; fewer blocks split the keys over more waves, so the GPU is
+// full with fewer tokens.  The count follows from the time that a shape would take, in us:
+//   a workgroup   3 before and after its keys, 0.35 per key tile for the copies (0.7: bf16), and 1.5 (two row-sets a wave)
+//                 or 1.64 (three) per key tile and wave;
+//   the grid      its rounds of 256 workgroups: whole ones where the blocks cost alike (a window, pairs); half a round of
+//                 the mean for the end otherwise, and not less than the longest workgroup.
+// Where the context is not the window's, the host knows the queries only and takes them for it: a block sees their
+// number at most, half of it on average.  Measured, us with 1 / 2 / 4 blocks (GQA 6 and 4): 4096 after 1000, window
+// 1024, 109 / 89 / 73; 5 of 100..1500, bf16, window 512, 114 / 83 / 64; 2048, window 512 58 / 43 / 35; 300, window 100
+// 12.6 / 16.6 / 18.8; whole contexts, 6 of 37..900 after 200 63 / 52 / 64, 2048 after 2048 at GQA 4 155 / 129 / 141, at
+// GQA 6 103 / 113 / 194.
+struct VisibleShape {
+    int rs, ng;
+};
+constexpr VisibleShape kVisibleShapes[] = {{2, 2}, {3, 2}, {2, 4}, {3, 4}, {2, 8}, {3, 8}};       // by row-sets
+
+struct VisiblePlan {
+    VisibleShape shape;
+    int nb, paired, ranks;             // ranks: workgroups per (sequence, kv head) of the longest sequence
+};
+
+// num_tokens: queries of all sequences, 0 where the caller did not say.
+VisiblePlan plan_visible(bool b16, int gqa, int hkv, int num_seqs, int max_query_len, int num_tokens, int window, int sinks)
 {
-    const int g = P.gqa;
-    if (g <= 2) launch_kernel(prefill_visible_kernel<2, 2, 2, false, true, SC>, grid, block, 0, stream, P);
-    else if (g <= 4) launch_kernel(prefill_visible_kernel<2, 2, 2, false, false, SC>, grid, block, 0, stream, P);
-    else if (g <= 6) launch_kernel(prefill_visible_kernel<3, 2, 2, false, false, SC>, grid, block, 0, stream, P);
-    else if (g <= 8) launch_kernel(prefill_visible_kernel<2, 4, 2, false, false, SC>, grid, block, 0, stream, P);
-    else if (g <= 12) launch_kernel(prefill_visible_kernel<3, 4, 2, false, false, SC>, grid, block, 0, stream, P);
-    else launch_kernel(prefill_visible_kernel<2, 8, 2, false, false, SC>, grid, block, 0, stream, P);
+    const double all = num_tokens > 0 ? num_tokens : (double)num_seqs * max_query_len;
+    const bool limited = window > 0 && window < max_query_len;
+    VisiblePlan best{};
+    double best_time = 1e300;
+    for (const VisibleShape s : kVisibleShapes) {
+        const int nb = s.rs * s.ng / gqa;
+        if (nb < 1) continue;
+        const double tile = (b16 ? 0.7 : 0.35) + (s.rs == 2 ? 1.5 : 1.64) * s.ng / kSplitWaves;
+        const double most = 3 + tile / kBN * (limited ? (double)window + sinks + 16 * nb : (double)max_query_len);
+        const double mean = limited ? most : 3 + tile / kBN * max_query_len / 2;
+        const int n = (max_query_len + 16 * nb - 1) / (16 * nb);
+        const double blocks = num_seqs == 1 ? n : all / (16 * nb) + num_seqs / 2.0;
+        const double wgs = hkv * (blocks > num_seqs ? blocks : num_seqs);
+        for (int paired = 0; paired < (limited ? 1 : 2); ++paired) {
+            const double x = wgs / (paired ? 2 : 1) / kSplitRoundWorkgroups;
+            double time = x <= 1 ? mean : limited || paired ? mean * ceil(x - 0.05) : mean * (x + 0.5);
+            if (paired) time *= 2;
+            else if (time < most) time = most;
+            if (time < best_time) {
+                best_time = time;
+                best = VisiblePlan{s, nb, paired, paired ? (n + 1) / 2 : n};
+            }
+        }
+    }
+    return best;
 }
 
-// Whole causal contexts: pairs of blocks (r, n - 1 - r) where single ones overflow a round of workgroups, as in
-// prefill_attn.hip.  With a window the blocks cost alike, and pairs would only halve the workgroups to
-// choose from.
-int launch_visible(const VisibleParams& P0, bool b16, int num_seqs, int max_query_len, hipStream_t stream)
+template <bool B16, bool SC>
+void launch_shape(const VisibleParams& P, VisibleShape s, dim3 grid, dim3 block, hipStream_t stream)
+{
+    constexpr int T = B16 ? 1 : 2;                     // tiles per wave and window, for windows of 64 KB
+    if (s.rs == 2) {
+        if (s.ng == 2) launch_kernel(prefill_visible_kernel<2, 2, T, B16, SC>, grid, block, 0, stream, P);
+        else if (s.ng == 4) launch_kernel(prefill_visible_kernel<2, 4, 2 * T, B16, SC>, grid, block, 0, stream, P);
+        else launch_kernel(prefill_visible_kernel<2, 8, 4 * T, B16, SC>, grid, block, 0, stream, P);
+    } else {
+        if (s.ng == 2) launch_kernel(prefill_visible_kernel<3, 2, T, B16, SC>, grid, block, 0, stream, P);
+        else if (s.ng == 4) launch_kernel(prefill_visible_kernel<3, 4, 2 * T, B16, SC>, grid, block, 0, stream, P);
+        else launch_kernel(prefill_visible_kernel<3, 8, 4 * T, B16, SC>, grid, block, 0, stream, P);
+    }
+}
+
+int launch_visible(const VisibleParams& P0, bool b16, int num_seqs, int max_query_len, int num_tokens, hipStream_t stream)
 {
     VisibleParams P = P0;
-    const int g = P.gqa;
-    P.nb = split_blocks(g);
-    const int n = (max_query_len + 16 * P.nb - 1) / (16 * P.nb);
+    const VisiblePlan L = plan_visible(b16, P.gqa, P.hkv, num_seqs, max_query_len, num_tokens, P.window, P.sinks);
+    P.nb = L.nb;
+    P.paired = L.paired;
     P.xcd_map = (P.hkv <= 8 && 8 % P.hkv == 0) ? 1 : 0;
-    P.paired = P.window == 0 && !split_single_blocks_fit(n, P.hkv, num_seqs);
-    const int per = split_xcd_per(P.hkv), ranks = P.paired ? (n + 1) / 2 : n;
-    P.ntb_grid = (ranks + per - 1) / per * per;
+    const int per = split_xcd_per(P.hkv);
+    P.ntb_grid = (L.ranks + per - 1) / per * per;
     const dim3 grid((unsigned)(P.ntb_grid * P.hkv), 1u, (unsigned)num_seqs), block(64 * kSplitWaves);
     begin_launch();
-    if (b16) {
-        if (g <= 2) launch_kernel(prefill_visible_kernel<2, 2, 1, true, true, false>, grid, block, 0, stream, P);
-        else if (g <= 4) launch_kernel(prefill_visible_kernel<2, 2, 1, true, false, false>, grid, block, 0, stream, P);
-        else if (g <= 6) launch_kernel(prefill_visible_kernel<3, 2, 1, true, false, false>, grid, block, 0, stream, P);
-        else if (g <= 8) launch_kernel(prefill_visible_kernel<2, 4, 2, true, false, false>, grid, block, 0, stream, P);
-        else launch_kernel(prefill_visible_kernel<2, 8, 4, true, false, false>, grid, block, 0, stream, P);
-    } else if (P.kv_scales) {
-        launch_e4m3<true>(P, grid, block, stream);
-    } else {
-        launch_e4m3<false>(P, grid, block, stream);
-    }
+    if (b16) launch_shape<true, false>(P, L.shape, grid, block, stream);
+    else if (P.kv_scales) launch_shape<false, true>(P, L.shape, grid, block, stream);
+    else launch_shape<false, false>(P, L.shape, grid, block, stream);
     return finish_launch();
 }
 
@@ -668,9 +732,10 @@ int prefill_visible(const void* q, int64_t q_row_stride, const void* k_cache, co
                     const int32_t* cu_seqlens_q, const int32_t* seq_lens, const int32_t* block_table, int64_t bt_stride,
                     const float* k_scale, const float* v_scale, const void* kv_scales, float sm_scale, int num_seqs,
                     int num_q_heads, int num_kv_heads, int head_size, int block_size, int window, int sinks,
-                    int max_query_len, void* stream)
+                    int max_query_len, int num_tokens, void* stream)
 {
-    if (!cu_seqlens_q || !seq_lens || num_seqs < 1 || max_query_len < 0 || window < 0 || sinks < 0) return FP8KV_ERR_ARG;
+    if (!cu_seqlens_q || !seq_lens || num_seqs < 1 || max_query_len < 0 || num_tokens < 0 || window < 0 || sinks < 0)
+        return FP8KV_ERR_ARG;
     if (KIND == kBlk && !kv_scales) return FP8KV_ERR_ARG;
     if (num_seqs > 65535) return FP8KV_ERR_SHAPE;
     const int64_t elem = KIND == kBf16 ? 2 : 1;
@@ -693,7 +758,7 @@ int prefill_visible(const void* q, int64_t q_row_stride, const void* k_cache, co
     P.kv_scales = static_cast<const uint16_t*>(kv_scales);
     P.window = window;
     P.sinks = sinks;
-    return launch_visible(P, KIND == kBf16, num_seqs, max_query_len, reinterpret_cast<hipStream_t>(stream));
+    return launch_visible(P, KIND == kBf16, num_seqs, max_query_len, num_tokens, reinterpret_cast<hipStream_t>(stream));
 }
 
 }  // namespace prefill_detail
@@ -707,11 +772,12 @@ extern "C" int fp8kv_prefill_attn_window(const void* q, int64_t q_row_stride, co
                                          const int32_t* seq_lens, const int32_t* block_table, int64_t bt_stride,
                                          const float* k_scale, const float* v_scale, float sm_scale, int num_seqs,
                                          int num_q_heads, int num_kv_heads, int head_size, int block_size, int window,
-                                         int sinks, int max_query_len, void* stream)
+                                         int sinks, int max_query_len, int num_tokens, void* stream)
 {
     return prefill_visible<kE4m3>(q, q_row_stride, k_cache, v_cache, sk0, sk1, sk2, sv0, sv1, sv2, out, out_row_stride,
                                   cu_seqlens_q, seq_lens, block_table, bt_stride, k_scale, v_scale, nullptr, sm_scale, num_seqs,
-                                  num_q_heads, num_kv_heads, head_size, block_size, window, sinks, max_query_len, stream);
+                                  num_q_heads, num_kv_heads, head_size, block_size, window, sinks, max_query_len, num_tokens,
+                                  stream);
 }
 
 extern "C" int fp8kv_prefill_attn_window_bf16(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
@@ -719,11 +785,12 @@ extern "C" int fp8kv_prefill_attn_window_bf16(const void* q, int64_t q_row_strid
                                               void* out, int64_t out_row_stride, const int32_t* cu_seqlens_q,
                                               const int32_t* seq_lens, const int32_t* block_table, int64_t bt_stride,
                                               float sm_scale, int num_seqs, int num_q_heads, int num_kv_heads, int head_size,
-                                              int block_size, int window, int sinks, int max_query_len, void* stream)
+                                              int block_size, int window, int sinks, int max_query_len, int num_tokens, void* stream)
 {
     return prefill_visible<kBf16>(q, q_row_stride, k_cache, v_cache, sk0, sk1, sk2, sv0, sv1, sv2, out, out_row_stride,
                                   cu_seqlens_q, seq_lens, block_table, bt_stride, nullptr, nullptr, nullptr, sm_scale, num_seqs,
-                                  num_q_heads, num_kv_heads, head_size, block_size, window, sinks, max_query_len, stream);
+                                  num_q_heads, num_kv_heads, head_size, block_size, window, sinks, max_query_len, num_tokens,
+                                  stream);
 }
 
 extern "C" int fp8kv_prefill_attn_blk(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
@@ -731,9 +798,22 @@ extern "C" int fp8kv_prefill_attn_blk(const void* q, int64_t q_row_stride, const
                                       void* out, int64_t out_row_stride, const int32_t* cu_seqlens_q, const int32_t* seq_lens,
                                       const int32_t* block_table, int64_t bt_stride, const void* kv_scales, float sm_scale,
                                       int num_seqs, int num_q_heads, int num_kv_heads, int head_size, int block_size,
-                                      int window, int sinks, int max_query_len, void* stream)
+                                      int window, int sinks, int max_query_len, int num_tokens, void* stream)
 {
     return prefill_visible<kBlk>(q, q_row_stride, k_cache, v_cache, sk0, sk1, sk2, sv0, sv1, sv2, out, out_row_stride,
                                  cu_seqlens_q, seq_lens, block_table, bt_stride, nullptr, nullptr, kv_scales, sm_scale, num_seqs,
-                                 num_q_heads, num_kv_heads, head_size, block_size, window, sinks, max_query_len, stream);
+                                 num_q_heads, num_kv_heads, head_size, block_size, window, sinks, max_query_len, num_tokens,
+                                  stream);
+}
+
+extern "C" int fp8kv_prefill_visible_plan(int num_q_heads, int num_kv_heads, int num_seqs, int max_query_len, int num_tokens,
+                                          int window, int sinks, int bf16, int* out)
+{
+    if (!out || num_q_heads < 1 || num_kv_heads < 1 || num_seqs < 1 || max_query_len < 0 || num_tokens < 0 || window < 0 || sinks < 0)
+        return FP8KV_ERR_ARG;
+    if (num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > kMaxGqa) return FP8KV_ERR_SHAPE;
+    const VisiblePlan L = plan_visible(bf16 != 0, num_q_heads / num_kv_heads, num_kv_heads, num_seqs, max_query_len, num_tokens, window, sinks);
+    const int v[5] = {L.shape.rs, L.shape.ng, L.nb, L.paired, L.ranks};
+    for (int i = 0; i < 5; ++i) out[i] = v[i];
+    return FP8KV_OK;
 }

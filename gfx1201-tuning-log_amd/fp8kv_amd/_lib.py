@@ -69,9 +69,9 @@ SIGNATURES: dict[str, tuple] = {
     "fp8kv_decode_attn_window": (_c_i, _DECODE + [_c_vp] * 2 + [_c_f] + [_c_i] * 6 + [_c_vp, _c_sz] + [_c_i] * 3 + [_c_vp]),
     "fp8kv_decode_attn_window_bf16": (_c_i, _DECODE + [_c_f] + [_c_i] * 6 + [_c_vp, _c_sz] + [_c_i] * 3 + [_c_vp]),
     "fp8kv_decode_attn_blk": (_c_i, _DECODE + [_c_vp, _c_f] + [_c_i] * 6 + [_c_vp, _c_sz] + [_c_i] * 3 + [_c_vp]),
-    "fp8kv_prefill_attn_window": (_c_i, _DECODE + [_c_vp] * 2 + [_c_f] + [_c_i] * 8 + [_c_vp]),
-    "fp8kv_prefill_attn_window_bf16": (_c_i, _DECODE + [_c_f] + [_c_i] * 8 + [_c_vp]),
-    "fp8kv_prefill_attn_blk": (_c_i, _DECODE + [_c_vp, _c_f] + [_c_i] * 8 + [_c_vp]),
+    "fp8kv_prefill_attn_window": (_c_i, _DECODE + [_c_vp] * 2 + [_c_f] + [_c_i] * 9 + [_c_vp]),
+    "fp8kv_prefill_attn_window_bf16": (_c_i, _DECODE + [_c_f] + [_c_i] * 9 + [_c_vp]),
+    "fp8kv_prefill_attn_blk": (_c_i, _DECODE + [_c_vp, _c_f] + [_c_i] * 9 + [_c_vp]),
     # position rotation and cache append in one pass (csrc/rope_append.hip)
     "fp8kv_rope_append": (_c_i, _ROPE_APPEND + [_c_vp] * 3 + [_c_i] * 5 + [_c_i64, _c_vp]),
     "fp8kv_rope_append_bf16": (_c_i, _ROPE_APPEND + [_c_vp] + [_c_i] * 5 + [_c_i64, _c_vp]),
@@ -106,6 +106,7 @@ SIGNATURES: dict[str, tuple] = {
     "fp8kv_prefill_bf16_tune": (None, [_c_i]),
     "fp8kv_prefill_plan": (_c_i, [_c_i, _c_i, _c_i, _c_i, _c_i, _c_vp]),
     "fp8kv_prefill_bf16_plan": (_c_i, [_c_i] * 5),
+    "fp8kv_prefill_visible_plan": (_c_i, [_c_i] * 8 + [_c_vp]),
     "fp8kv_gemm_tune": (None, [_c_i, _c_i]),
     "fp8kv_gemm_plan": (_c_i, [_c_i] * 4),
     "fp8kv_time_next_launch": (None, [_c_vp, _c_vp]),

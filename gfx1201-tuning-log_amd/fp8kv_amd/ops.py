@@ -607,11 +607,11 @@ def prefill_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     if max_query_len is None:
         max_query_len = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item())
     if bf16:
-        _launch("fp8kv_prefill_attn_window_bf16", dev, *lead, sm_scale, *geometry, window, sinks, max_query_len)
+        _launch("fp8kv_prefill_attn_window_bf16", dev, *lead, sm_scale, *geometry, window, sinks, max_query_len, q.shape[0])
     else:
         ks, vs = _scale_tensor(k_scale, q.device), _scale_tensor(v_scale, q.device)
         _launch("fp8kv_prefill_attn_window", dev, *lead, ks.data_ptr(), vs.data_ptr(), sm_scale, *geometry, window, sinks,
-                max_query_len)
+                max_query_len, q.shape[0])
     return out
 
 
@@ -644,7 +644,7 @@ def prefill_attention_blk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         return out
     if max_query_len is None:
         max_query_len = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item())
-    _launch("fp8kv_prefill_attn_blk", dev, *lead, scales, sm_scale, *geometry, window, sinks, max_query_len)
+    _launch("fp8kv_prefill_attn_blk", dev, *lead, scales, sm_scale, *geometry, window, sinks, max_query_len, q.shape[0])
     return out
 
 

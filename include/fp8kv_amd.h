@@ -289,7 +289,8 @@ int fp8kv_prefill_attn_varlen_bf16(const void* q, int64_t q_row_stride,
  * decode: one query per sequence, at position seq_lens[s] - 1; prefill: the packed sequences of
  * fp8kv_prefill_attn_varlen, row i of sequence s at position seq_lens[s] - qlen_s + i.  Layouts, strides, geometry limits,
  * splits, scratch and max_seq_len as for fp8kv_decode_attn_ctx and fp8kv_prefill_attn_varlen (bf16: as for their bf16
- * forms); fp8kv_decode_num_splits is asked with the longest visible set, min(max_seq_len, window + sinks).
+ * forms); num_tokens is the number of queries of all sequences, for the launch plan alone (0: not known);
+ * fp8kv_decode_num_splits is asked with the longest visible set, min(max_seq_len, window + sinks).
  *   - Block-table entries of blocks without a visible key are never used, whatever they hold, so blocks that the
  *     window has left can be given back.
  *   - Rows that see nothing are zeros: seq_lens[s] <= 0, and rows of negative position (seq_lens[s] < qlen_s).
@@ -331,7 +332,8 @@ int fp8kv_prefill_attn_window(const void* q, int64_t q_row_stride,
                               const int32_t* block_table, int64_t bt_stride,
                               const float* k_scale, const float* v_scale, float sm_scale,
                               int num_seqs, int num_q_heads, int num_kv_heads, int head_size,
-                              int block_size, int window, int sinks, int max_query_len, void* stream);
+                              int block_size, int window, int sinks, int max_query_len, int num_tokens,
+                              void* stream);
 
 int fp8kv_prefill_attn_window_bf16(const void* q, int64_t q_row_stride,
                                    const void* k_cache, const void* v_cache,
@@ -342,7 +344,8 @@ int fp8kv_prefill_attn_window_bf16(const void* q, int64_t q_row_stride,
                                    const int32_t* block_table, int64_t bt_stride,
                                    float sm_scale,
                                    int num_seqs, int num_q_heads, int num_kv_heads, int head_size,
-                                   int block_size, int window, int sinks, int max_query_len, void* stream);
+                                   int block_size, int window, int sinks, int max_query_len, int num_tokens,
+                              void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Attention over a block-scaled cache (fp8kv_rope_append_blk): e4m3 codes with one power-of-two scale per 16
@@ -372,7 +375,8 @@ int fp8kv_prefill_attn_blk(const void* q, int64_t q_row_stride,
                            const int32_t* block_table, int64_t bt_stride,
                            const void* kv_scales, float sm_scale,
                            int num_seqs, int num_q_heads, int num_kv_heads, int head_size,
-                           int block_size, int window, int sinks, int max_query_len, void* stream);
+                           int block_size, int window, int sinks, int max_query_len, int num_tokens,
+                              void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * fp8-e4m3 KV-cache write: quantise new K and V rows and scatter them into the paged cache.

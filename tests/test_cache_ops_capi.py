@@ -107,14 +107,14 @@ def test_visible_attention_rejects_before_launch(lib, change, code):
             change = dict(_5=260)
         args = _att(elem, **change)
         assert dec(*args, *scales, 0.1, *GEO, 4, None, 0, 64, 4, 0, None) == code
-        assert pre(*args, *scales, 0.1, *GEO, 64, 4, 0, None) == code
+        assert pre(*args, *scales, 0.1, *GEO, 64, 4, 0, 0, None) == code
 
 
 @pytest.mark.parametrize("geo,code", GEO_CHECKS)
 def test_visible_attention_geometry(lib, geo, code):
     for dec, pre, elem, scales in _forms(lib):
         assert dec(*_att(elem), *scales, 0.1, *geo, 4, None, 0, 64, 4, 0, None) == code
-        assert pre(*_att(elem), *scales, 0.1, *geo, 64, 4, 0, None) == code
+        assert pre(*_att(elem), *scales, 0.1, *geo, 64, 4, 0, 0, None) == code
 
 
 def test_visible_attention_window_splits_and_scales(lib):
@@ -122,18 +122,19 @@ def test_visible_attention_window_splits_and_scales(lib):
         args = _att(elem)
         for win in ((-1, 0), (0, -1)):
             assert dec(*args, *scales, 0.1, *GEO, 1, None, 0, *win, 0, None) == 1
-            assert pre(*args, *scales, 0.1, *GEO, *win, 0, None) == 1
+            assert pre(*args, *scales, 0.1, *GEO, *win, 0, 0, None) == 1
         assert dec(*args, *scales, 0.1, *GEO, 0, None, 0, 64, 4, 0, None) == 1
         assert dec(*args, *scales, 0.1, *GEO, 257, None, 0, 64, 4, 0, None) == 1
         assert dec(*args, *scales, 0.1, *GEO, 4, A, 100, 64, 4, 0, None) == 5
-        assert pre(*args, *scales, 0.1, *GEO, 64, 4, -1, None) == 1
+        assert pre(*args, *scales, 0.1, *GEO, 64, 4, -1, 0, None) == 1
+        assert pre(*args, *scales, 0.1, *GEO, 64, 4, 0, -1, None) == 1
         for i in range(len(scales)):
             missing = scales[:i] + [None] + scales[i + 1:]
             assert dec(*args, *missing, 0.1, *GEO, 1, None, 0, 64, 4, 0, None) == 1
-            assert pre(*args, *missing, 0.1, *GEO, 64, 4, 0, None) == 1
-        assert pre(*args, *scales, 0.1, *GEO, 64, 4, 0, None) == 0                    # no queries: nothing is launched
+            assert pre(*args, *missing, 0.1, *GEO, 64, 4, 0, 0, None) == 1
+        assert pre(*args, *scales, 0.1, *GEO, 64, 4, 0, 0, None) == 0                    # no queries: nothing is launched
     assert lib.fp8kv_decode_attn_blk(*_att(), A + 1, 0.1, *GEO, 1, None, 0, 64, 4, 0, None) == 3
-    assert lib.fp8kv_prefill_attn_blk(*_att(), A + 1, 0.1, *GEO, 64, 4, 0, None) == 3
+    assert lib.fp8kv_prefill_attn_blk(*_att(), A + 1, 0.1, *GEO, 64, 4, 0, 0, None) == 3
 
 
 # ---- the oracle itself ---------------------------------------------------------------------------
