@@ -70,6 +70,30 @@ __device__ __forceinline__ float add_bf16x2(uint32_t w, float l)
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), __builtin_bit_cast(bf16x2_t, 0x3F803F80u), l, false);
 }
 
+// What a weight may grow to before its row's reference moves, and how far above the row's max it moves then, in log2: a
+// row whose max then grows by less than the sum of the two is left alone, at weights between 2^-kLift and 2^kCeil.
+constexpr float kCeil = 256.f, kLift = 8.f;
+
+// New references and accumulators of RS row-sets after a weight past kCeil, from the tile's raw scores.
+template <int RS>
+__device__ __forceinline__ void lift_rows(const f32x4_t (&sc)[RS][2], float (&m_run)[RS], float (&l_run)[RS],
+                                          f32x4_t (&o)[RS][8], const float (&qkr)[RS])
+{
+#pragma unroll
+    for (int j = 0; j < RS; ++j) {
+        float m = max3_raw(sc[j][0][0], sc[j][0][1], sc[j][0][2]);
+        m = max3_raw(m, sc[j][0][3], sc[j][1][0]);
+        m = max3_raw(m, sc[j][1][1], sc[j][1][2]);
+        const float mc = max_xor16_32_raw(max_raw(m, sc[j][1][3])) * qkr[j];      // -inf for a fully masked row
+        const float m_new = mc > m_run[j] ? mc + kLift : m_run[j];
+        const float alpha = __builtin_amdgcn_exp2f(m_run[j] - m_new);
+        l_run[j] *= alpha;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) o[j][n] *= alpha;
+        m_run[j] = m_new;
+    }
+}
+
 // SC: block-scaled e4m3 caches.
 template <int RS, int NG, int TPW, bool B16, bool SC>
 __global__ void __launch_bounds__(kSplitWaves * 64)
@@ -389,6 +413,21 @@ prefill_visible_kernel(VisibleParams P)
                     }
                 }
                 [[maybe_unused]] u32x4_t vf[8];
+                [[maybe_unused]] u32x2_t vr[8];
+                [[maybe_unused]] float vsc[2] = {1.f, 1.f};
+                // V^T fragments 4 w .. 4 w + 3 (d = 8c + 4w ..) from word w of the raw rows, as v_fragments
+                auto widen = [&](int w) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t x = __builtin_amdgcn_perm(vr[2 * k + 1][w], vr[2 * k][w], 0x05010400u);   // a0 b0 a1 b1
+                        const uint32_t y = __builtin_amdgcn_perm(vr[2 * k + 1][w], vr[2 * k][w], 0x07030602u);   // a2 b2 a3 b3
+                        const float f = vsc[k >> 1];
+                        vf[4 * w + 0][k] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, f, false));
+                        vf[4 * w + 1][k] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, f, true));
+                        vf[4 * w + 2][k] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, f, false));
+                        vf[4 * w + 3][k] = bf16x2_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, f, true));
+                    }
+                };
                 if constexpr (!B16) {
                     v8i kf[2];
 #pragma unroll
@@ -399,15 +438,14 @@ prefill_visible_kernel(VisibleParams P)
                                        (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
                     }
                     uint32_t scales = 127 | 127 << 16;
-                    float vsc[2] = {1.f, 1.f};
                     if constexpr (SC) {
                         scales = *reinterpret_cast<const uint32_t*>(lds_scales[i & 1][tw]);
                         const uint32_t u = __builtin_amdgcn_readfirstlane(scales);
                         vsc[0] = __uint_as_float((u & 0xFF00u) << 15);         // bytes 1 .. 254 are exponents as they are
                         vsc[1] = __uint_as_float((u & 0xFF000000u) >> 1);
                     }
-                    // V^T raw rows (lane (c, p) transposes d = 8c .. 8c+7) and their widening go ahead of S^T = K.Q^T
-                    u32x2_t vr[8];
+                    // V^T raw rows (lane (c, p) transposes d = 8c .. 8c+7) and the widening of their first half go along
+                    // with S^T = K.Q^T
 #pragma unroll
                     for (int jj = 0; jj < 8; ++jj) {
                         vr[jj] = *reinterpret_cast<const u32x2_t*>(buf + v_lane + 256 * (jj & 3) + (jj < 4 ? 0 : 2048));
@@ -426,7 +464,7 @@ prefill_visible_kernel(VisibleParams P)
                             }
                         }
                     }
-                    v_fragments(vr, vf, vsc[0], vsc[1]);
+                    widen(0);
 #pragma unroll
                     for (int j = 0; j < RS; ++j) {
                         const f32x4_t zero = {0.f, 0.f, 0.f, 0.f};
@@ -435,11 +473,13 @@ prefill_visible_kernel(VisibleParams P)
                         acc = score_mfma<1, false>(kf[1], qhi[j], zero, scales);
                         sc[j][1] = score_mfma<1, true>(kf[1], qlo[j], acc, scales);
                     }
-                    // Interleave: one MFMA, then up to four VALU (the V widening, 48 instructions).
+                    // pinned here, where the vector units would wait: one MFMA, then two or three of its 24 instructions
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) asm volatile("" : "+v"(vf[n]));
 #pragma unroll
                     for (int g = 0; g < 4 * RS; ++g) {
                         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 24 / (4 * RS), 0);
                     }
                 }
                 if (masked) {
@@ -458,39 +498,54 @@ prefill_visible_kernel(VisibleParams P)
                             }
                     }
                 }
-                rescale_rows<RS>(sc, m_run, l_run, o, qkr);
-                // Weights of row-set j in bf16 (the P^T operand).  The max is a rounded product and the fused difference is
-                // not, so where scores are past 10^7 the largest weight is not 1 but 2^+-(half a unit in the max's last
-                // place): nothing to bf16 and its fp32 sums.
-                auto row_weights = [&](int j) -> u32x4_t {
-                    u32x4_t pb;
+                // Weights of row-set j in bf16 (the P^T operand) and their sum.  The reference is a rounded product and the
+                // fused difference is not, so where scores are past 10^7 a row's largest weight is off by 2^+-(half a unit in
+                // the reference's last place): nothing to bf16 and its fp32 sums.
+                u32x4_t pb[RS];
+                float ps[RS];
+                auto row_weights = [&](int j) {
 #pragma unroll
                     for (int d = 0; d < 4; ++d) {
                         const f32x4_t& x = sc[j][d >> 1];
-                        pb[d] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (d & 1)], qkr[j], -m_run[j])),
-                                            __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (d & 1) + 1], qkr[j], -m_run[j])));
+                        pb[j][d] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (d & 1)], qkr[j], -m_run[j])),
+                                               __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (d & 1) + 1], qkr[j], -m_run[j])));
                     }
-                    l_run[j] = add_bf16x2(pb[3], add_bf16x2(pb[2], add_bf16x2(pb[1], add_bf16x2(pb[0], l_run[j]))));
-                    return pb;
+                    ps[j] = add_bf16x2(pb[j][3], add_bf16x2(pb[j][2], add_bf16x2(pb[j][1], add_bf16x2(pb[j][0], 0.f))));
                 };
+                // The sums tell whether a weight grew past kCeil (or eight of them together): then the references move and the
+                // weights are formed again.  Looking for the row maxima first costs 24 instructions a tile and one more
+                // dependent step, for something that happens at the start of a row and hardly ever after.
+                bool over = false;
+#pragma unroll
+                for (int j = 0; j < RS; ++j) {
+                    row_weights(j);
+                    over |= ps[j] > kCeil;
+                }
+                if (__any(over)) {
+                    lift_rows<RS>(sc, m_run, l_run, o, qkr);
+#pragma unroll
+                    for (int j = 0; j < RS; ++j) row_weights(j);
+                }
+#pragma unroll
+                for (int j = 0; j < RS; ++j) l_run[j] += ps[j];
                 if constexpr (!B16) {
+                    // the first half of d, and the second half's widening beside it
 #pragma unroll
-                    for (int j = 0; j < RS; ++j) {
-                        const u32x4_t pb = row_weights(j);
+                    for (int n = 0; n < 4; ++n)
 #pragma unroll
-                        for (int n = 0; n < 8; ++n) o[j][n] = mfma16x16x32_bf16(as_bf16x8(vf[n]), as_bf16x8(pb), o[j][n]);
-                    }
-                    // Interleave: the first row-set's exponentials alone, then each P.V MFMA with three
-                    // VALU instructions of the next row-set's softmax.
-                    __builtin_amdgcn_sched_group_barrier(0x002, 24, 0);
+                        for (int j = 0; j < RS; ++j) o[j][n] = mfma16x16x32_bf16(as_bf16x8(vf[n]), as_bf16x8(pb[j]), o[j][n]);
+                    widen(1);
 #pragma unroll
-                    for (int g = 0; g < 8 * (RS - 1); ++g) {
+                    for (int n = 4; n < 8; ++n)
+#pragma unroll
+                        for (int j = 0; j < RS; ++j) o[j][n] = mfma16x16x32_bf16(as_bf16x8(vf[n]), as_bf16x8(pb[j]), o[j][n]);
+#pragma unroll
+                    for (int g = 0; g < 4 * RS; ++g) {
                         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 24 / (4 * RS), 0);
                     }
                 } else {
                     // Half of a V row's 16 bytes at a time: half h is d = 8c + 4h .. + 3.
-                    u32x2_t vr[8];
                     auto read_half = [&](int h) {
 #pragma unroll
                         for (int jj = 0; jj < 8; ++jj) {
@@ -506,9 +561,6 @@ prefill_visible_kernel(VisibleParams P)
                         }
                     };
                     read_half(0);
-                    u32x4_t pb[RS];
-#pragma unroll
-                    for (int j = 0; j < RS; ++j) pb[j] = row_weights(j);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         u32x4_t va[4];
