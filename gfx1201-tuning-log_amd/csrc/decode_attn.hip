@@ -91,6 +91,7 @@ struct Params {
 struct VisibleParams : Params {
     const uint16_t* kv_scales;      // block-scaled caches: [blocks][block_size / 16][hkv] pairs of e8m0 bytes
     int window, sinks;
+    int ns, parts;                  // sequences; parts that their walks are cut into (kv_visible.h), 0: none
 };
 
 // Floats per split record, rounded up to a multiple of four so that every record starts 16-byte
@@ -114,11 +115,10 @@ __host__ __device__ inline void split_span(int seqlen, int nsplit, int sp, int& 
 // the last split); the wave reads the pairs with readlane, computes the factors exp2(m_s - max m)
 // once for both elements, and adds every split's term independently of the others.
 template <int SMAX, int T>
-__device__ __forceinline__ void merge_regs(const Params& P, const float* recs, int rf, int E, int tid, float vs,
+__device__ __forceinline__ void merge_regs(const Params& P, const float* recs, int ns, int rf, int E, int tid, float vs,
                                             int64_t out_row)
 {
     static_assert(SMAX <= 64, "one (m, l) pair per lane");
-    const int ns = P.nsplit;
     const int lane = tid & 63;
     const int sl = lane < ns ? lane : ns - 1;
     for (int e0 = 0; e0 < E; e0 += 2 * T) {
@@ -164,7 +164,8 @@ __device__ __forceinline__ void merge_regs(const Params& P, const float* recs, i
 // requested together with the rest of P instead of after it.
 // The kernel body, for e4m3 or bf16 K/V caches over whole contexts (PT = Params), or for the visible keys of
 // any cache kind (PT = VisibleParams, kv_visible.h).
-template <int W, int NG, int DEPTH, bool KF, int KIND, typename PT>
+// PARTS: workgroup x of a kv head takes part x of the batch (kv_visible.h), not split x of sequence z.
+template <int W, int NG, int DEPTH, bool KF, int KIND, bool PARTS, typename PT>
 __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens, const int32_t* __restrict__ qsl,
                                             const PT& P)
 {
@@ -196,21 +197,54 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
     __shared__ int lds_last;
     static_assert(W * kMaxGqa * kD >= 2 * kMaxSplits * kMaxGqa, "merge statistics must fit in lds_o");
 
-    const int sp = blockIdx.x, kh = blockIdx.y, seq = blockIdx.z;
-    const int tid = threadIdx.x;
+    int sp = blockIdx.x, seq = blockIdx.z;
+    const int kh = blockIdx.y;
+    const int gqa = P.gqa;
+    [[maybe_unused]] Part part;
+    if constexpr (PARTS) {
+        part = find_part(seq_lens, P.ns, P.parts, blockIdx.x, P.window, P.sinks, threadIdx.x & 63);
+        if (part.size == 0) return;                    // more parts than groups
+        seq = part.seq;
+        seqlen = part.len;
+        qtok = ((const_i32_t*)qsl)[seq];
+    }
+    // One segment: a split of one sequence, or what a part holds of one of its sequences.
+    for (;;) {
+    int tid = threadIdx.x;
+    if constexpr (PARTS) asm volatile("" : "+v"(tid));          // nothing that follows from it is kept between segments
     const int lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lr = lane & 15;
     const int lp = lane >> 4;
-    const int gqa = P.gqa;
 
     int lo, hi;
+    int64_t rec0;                                      // where the split records of this (sequence, kv head) start,
+    int nrec;                                          // and how many there are
     [[maybe_unused]] Walk walk;
+    [[maybe_unused]] int next_len = 0, next_tok = 0, groups = 0;
     if constexpr (VISIBLE) {
         walk = make_walk(seqlen, P.window, P.sinks);
-        split_span(walk.nv, nsplit, sp, lo, hi);
+    }
+    if constexpr (PARTS) {
+        const int next = seq + 1 < P.ns ? seq + 1 : seq;
+        next_len = ((const_i32_t*)seq_lens)[next];
+        next_tok = ((const_i32_t*)qsl)[next];
+        groups = walk_groups(walk.nv);
+        const int w = blockIdx.x, end = part.start + part.size;
+        lo = part.start > part.base ? 16 * (part.start - part.base) : 0;
+        hi = end - part.base < groups ? 16 * (end - part.base) : walk.nv;
+        const int first = part.base >= part.start ? w : (int)((unsigned)part.base / (unsigned)part.size);
+        const int past = part.base + groups <= end ? w : (int)((unsigned)(part.base + groups - 1) / (unsigned)part.size);
+        sp = w - first;
+        nrec = past - first + 1;
+        // A record's place counts the parts and the sequences before it.
+        rec0 = (int64_t)kh * (P.parts + P.ns) + first + seq;
     } else {
-        split_span(seqlen, nsplit, sp, lo, hi);
+        int tokens = seqlen;
+        if constexpr (VISIBLE) tokens = walk.nv;
+        split_span(tokens, nsplit, sp, lo, hi);
+        nrec = P.nsplit;
+        rec0 = ((int64_t)seq * P.hkv + kh) * nrec;
     }
     // The three steps of a chunk: its block ids, its loads, its use.
     auto ids_of = [&](const int32_t* row, int c0, int end) {
@@ -346,7 +380,8 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
         }
         mx = m;
     };
-    if (P.nsplit == 1) {
+    auto finish = [&] {
+    if (nrec == 1) {
         for (int e0 = 0; e0 < E; e0 += 4 * T) {
             const int e = e0 + 4 * tid;
             if (e >= E) break;
@@ -364,7 +399,7 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
 
     // ---- this split's partial record -------------------------------------------------------------
     const int rf = record_floats(gqa);
-    float* rec = P.part + (pair * P.nsplit + sp) * rf;
+    float* rec = P.part + (rec0 + sp) * rf;
     for (int e0 = 0; e0 < E; e0 += 4 * T) {
         const int e = e0 + 4 * tid;
         if (e >= E) break;
@@ -384,24 +419,24 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
     if (tid == 0) {
         const uint32_t t = __hip_atomic_fetch_add(P.counters + ticket_slot(pair), 1u, __ATOMIC_RELAXED,
                                                   __HIP_MEMORY_SCOPE_AGENT);
-        lds_last = (t == (uint32_t)(P.nsplit - 1)) ? 1 : 0;
+        lds_last = (t == (uint32_t)(nrec - 1)) ? 1 : 0;
     }
     __syncthreads();
     if (!lds_last) return;
 
-    const float* recs_all = P.part + pair * P.nsplit * rf;
+    const float* recs_all = P.part + rec0 * rf;
     const int64_t out_row = (int64_t)qtok * P.o_stride + (int64_t)(kh * gqa) * kD;
-    if (P.nsplit <= 32) {
-        if (P.nsplit <= 2)
-            merge_regs<2, T>(P, recs_all, rf, E, tid, vs, out_row);
-        else if (P.nsplit <= 4)
-            merge_regs<4, T>(P, recs_all, rf, E, tid, vs, out_row);
-        else if (P.nsplit <= 8)
-            merge_regs<8, T>(P, recs_all, rf, E, tid, vs, out_row);
-        else if (P.nsplit <= 16)
-            merge_regs<16, T>(P, recs_all, rf, E, tid, vs, out_row);
+    if (nrec <= 32) {
+        if (nrec <= 2)
+            merge_regs<2, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+        else if (nrec <= 4)
+            merge_regs<4, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+        else if (nrec <= 8)
+            merge_regs<8, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+        else if (nrec <= 16)
+            merge_regs<16, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
         else
-            merge_regs<32, T>(P, recs_all, rf, E, tid, vs, out_row);
+            merge_regs<32, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
         if (tid == 0)
             __hip_atomic_store(P.counters + ticket_slot(pair), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         return;
@@ -411,20 +446,20 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
     // splits: m and l of every split go to LDS once
     // (one load per split and head), each thread loads the o values of its own elements
     // tid + T j, and both are in flight together before the barrier.
-    const float* recs = P.part + pair * P.nsplit * rf;
-    const int NSG = P.nsplit * gqa;
+    const float* recs = P.part + rec0 * rf;
+    const int NSG = nrec * gqa;
     float* wm = &lds_o[0][0][0];            // [nsplit][gqa] m, then [nsplit][gqa] l
     float m[EPT], acc[EPT], l[EPT];
 #pragma unroll
     for (int j = 0; j < EPT; ++j) { m[j] = neg_inf(); acc[j] = 0.f; l[j] = 0.f; }
-    for (int s0 = 0; s0 < P.nsplit; s0 += kMergeBatch) {
+    for (int s0 = 0; s0 < nrec; s0 += kMergeBatch) {
         float ov[EPT][kMergeBatch];
 #pragma unroll
         for (int j = 0; j < EPT; ++j) {
             const int e = tid + T * j;
 #pragma unroll
             for (int b = 0; b < kMergeBatch; ++b) {
-                const int s2 = s0 + b < P.nsplit ? s0 + b : P.nsplit - 1;
+                const int s2 = s0 + b < nrec ? s0 + b : nrec - 1;
                 ov[j][b] = e < E ? load_coherent(recs + (int64_t)s2 * rf + e) : 0.f;
             }
         }
@@ -442,7 +477,7 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
             if (h >= gqa) continue;
 #pragma unroll
             for (int b = 0; b < kMergeBatch; ++b) {
-                if (s0 + b >= P.nsplit) break;
+                if (s0 + b >= nrec) break;
                 const float ms = wm[(s0 + b) * gqa + h];
                 const float mn = fmaxf(m[j], ms);
                 const float mu = mn == neg_inf() ? 0.f : mn;
@@ -464,13 +499,26 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
     }
     if (tid == 0)
         __hip_atomic_store(P.counters + ticket_slot(pair), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+    finish();
+    if constexpr (PARTS) {
+        part.base += groups;
+        ++seq;
+        if (part.base >= part.start + part.size || seq >= P.ns) return;
+        seqlen = next_len;
+        qtok = next_tok;
+        __syncthreads();                               // the next segment's states go where this one's were read
+    } else {
+        return;
+    }
+    }
 }
 
 template <int W, int NG, int DEPTH, bool KF>
 __global__ void __launch_bounds__(W * 64)
 decode_kernel(const int32_t* __restrict__ seq_lens, const int32_t* __restrict__ qsl, Params P)
 {
-    decode_body<W, NG, DEPTH, KF, kE4m3>(seq_lens, qsl, P);
+    decode_body<W, NG, DEPTH, KF, kE4m3, false>(seq_lens, qsl, P);
 }
 
 // bf16 K/V caches: the same kernel with twice the bytes per chunk and no widening (the reference's
@@ -479,15 +527,15 @@ template <int W, int NG, int DEPTH, bool KF>
 __global__ void __launch_bounds__(W * 64)
 decode_bf16kv_kernel(const int32_t* __restrict__ seq_lens, const int32_t* __restrict__ qsl, Params P)
 {
-    decode_body<W, NG, DEPTH, KF, kBf16>(seq_lens, qsl, P);
+    decode_body<W, NG, DEPTH, KF, kBf16, false>(seq_lens, qsl, P);
 }
 
 // The visible keys of a window and the first tokens, over caches of any kind, and block-scaled caches whole.
-template <int W, int NG, int DEPTH, bool KF, int KIND>
+template <int W, int NG, int DEPTH, bool KF, int KIND, bool PARTS>
 __global__ void __launch_bounds__(W * 64)
 decode_visible_kernel(const int32_t* __restrict__ seq_lens, const int32_t* __restrict__ qsl, VisibleParams P)
 {
-    decode_body<W, NG, DEPTH, KF, KIND>(seq_lens, qsl, P);
+    decode_body<W, NG, DEPTH, KF, KIND, PARTS>(seq_lens, qsl, P);
 }
 
 inline size_t counters_bytes() { return (size_t)kMaxPairs * sizeof(uint32_t); }
@@ -737,17 +785,52 @@ inline int visible_len(int max_seq_len, int window, int sinks)
     return max_seq_len <= 0 || max_seq_len > most ? (int)(most < kUnknownContext ? most : kUnknownContext) : max_seq_len;
 }
 
-template <int KIND>
-int launch_visible(const VisibleParams& P, int num_seqs, int max_seq_len, hipStream_t st)
+// Equal parts of the whole batch instead of splits of each sequence (kv_visible.h), one for each CU: pays where what a
+// CU waits for at the end of a ragged batch is more than the segments that a part begins with, 4 to 5 us each.  In
+// tokens of e4m3 (bf16: twice as many), a sequence is long from 2048 on, and the batch from 2560 per CU, or
+// half of that where the pairs do not divide the CUs.  Time against the planned splits, 1/8 to 1 of the longest and
+// nearly equal: 32 x 8 pairs of 2048 1.21 1.13, 4096 0.88 1.10, 8192 0.78 1.01; 16 x 4 of 4096 1.07 1.19, 16384
+// 0.79 1.02; 24 x 8 of 1024 1.32 1.22, 2048 0.90 0.83, 8192 0.81 0.80; 64 x 8 of 1024 1.08 1.14, 2048 0.94 1.06, 8192 0.79
+// 0.98; 128 x 8 of 1024 1.27 1.17, 4096 0.87 0.96; bf16 32 x 8 of 1024 1.18 1.22, 2048 0.95 1.09, 24 x 8 of 1024 0.94
+// 0.93.  Two parts per CU are 3 to 8 % slower on long contexts.
+constexpr int kLongWalk = 2048, kShareTokens = 2560;
+
+// Parts per kv head, or 0 for splits.
+inline int plan_parts(int ns, int hkv, int len, bool bf16)
 {
+    const int64_t tokens = (int64_t)len * (bf16 ? 2 : 1), pairs = (int64_t)ns * hkv;
+    if (ns < 2 || ns > kMaxShared || hkv > kCus || tokens < kLongWalk || len >= kUnknownContext) return 0;
+    const int64_t most = (int64_t)kCus * (pairs <= kCus && kCus % pairs == 0 ? kShareTokens : kShareTokens / 2);
+    return pairs * tokens < most ? 0 : kCus / hkv;
+}
+
+// The parts of a call with scratch for nsplit splits: a record for every part and sequence.
+inline int fit_parts(int parts, int ns, int nsplit)
+{
+    const int64_t most = (int64_t)(nsplit - 1) * ns;
+    return parts < most ? parts : (int)most;
+}
+
+template <int KIND>
+int launch_visible(VisibleParams& P, int num_seqs, int max_seq_len, hipStream_t st)
+{
+    const int len = visible_len(max_seq_len, P.window, P.sinks);
+    P.ns = num_seqs;
+    P.parts = fit_parts(plan_parts(num_seqs, P.hkv, len, KIND == kBf16), num_seqs, P.nsplit);
     const dim3 grid((unsigned)P.nsplit, (unsigned)P.hkv, (unsigned)num_seqs), block(8 * 64);
     begin_launch();
-    if constexpr (KIND == kBf16) {
-        launch_kernel(decode_visible_kernel<8, 2, 2, true, KIND>, grid, block, 0, st, P.seq_lens, P.qsl, P);
-    } else if (pick_variant((int64_t)P.nsplit * P.hkv * num_seqs, P.nsplit, visible_len(max_seq_len, P.window, P.sinks)) == 1) {
-        launch_kernel(decode_visible_kernel<8, 2, 1, false, KIND>, grid, block, 0, st, P.seq_lens, P.qsl, P);
+    if (P.parts > 0) {
+        const dim3 shared((unsigned)P.parts, (unsigned)P.hkv);
+        if constexpr (KIND == kBf16)
+            launch_kernel(decode_visible_kernel<8, 2, 2, true, KIND, true>, shared, block, 0, st, P.seq_lens, P.qsl, P);
+        else
+            launch_kernel(decode_visible_kernel<8, 2, 1, false, KIND, true>, shared, block, 0, st, P.seq_lens, P.qsl, P);
+    } else if constexpr (KIND == kBf16) {
+        launch_kernel(decode_visible_kernel<8, 2, 2, true, KIND, false>, grid, block, 0, st, P.seq_lens, P.qsl, P);
+    } else if (pick_variant((int64_t)P.nsplit * P.hkv * num_seqs, P.nsplit, len) == 1) {
+        launch_kernel(decode_visible_kernel<8, 2, 1, false, KIND, false>, grid, block, 0, st, P.seq_lens, P.qsl, P);
     } else {
-        launch_kernel(decode_visible_kernel<8, 2, 2, false, KIND>, grid, block, 0, st, P.seq_lens, P.qsl, P);
+        launch_kernel(decode_visible_kernel<8, 2, 2, false, KIND, false>, grid, block, 0, st, P.seq_lens, P.qsl, P);
     }
     return finish_launch();
 }
@@ -811,6 +894,15 @@ extern "C" int fp8kv_decode_num_splits_bf16(int num_seqs, int num_kv_heads, int 
 {
     if (num_seqs < 1 || num_kv_heads < 1) return 1;
     return plan_splits(num_seqs, num_kv_heads, max_seq_len, true);
+}
+
+extern "C" int fp8kv_decode_visible_splits(int num_seqs, int num_kv_heads, int max_seq_len, int window, int sinks, int bf16)
+{
+    if (num_seqs < 1 || num_kv_heads < 1 || window < 0 || sinks < 0) return 1;
+    const int len = visible_len(max_seq_len, window, sinks);
+    const int parts = plan_parts(num_seqs, num_kv_heads, len, bf16 != 0);
+    if (parts > 0) return (parts + num_seqs - 1) / num_seqs + 1;
+    return plan_splits(num_seqs, num_kv_heads, len, bf16 != 0);
 }
 
 extern "C" size_t fp8kv_decode_scratch_bytes(int num_seqs, int num_q_heads, int num_kv_heads,

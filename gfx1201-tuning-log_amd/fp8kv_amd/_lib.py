@@ -66,6 +66,7 @@ SIGNATURES: dict[str, tuple] = {
                           + [_c_vp] * 3 + [_c_i] * 4 + [_c_vp]),
     # attention over the visible keys of a window, and over block-scaled caches (csrc/decode_attn.hip,
     # csrc/prefill_visible.hip)
+    "fp8kv_decode_visible_splits": (_c_i, [_c_i] * 6),
     "fp8kv_decode_attn_window": (_c_i, _DECODE + [_c_vp] * 2 + [_c_f] + [_c_i] * 6 + [_c_vp, _c_sz] + [_c_i] * 3 + [_c_vp]),
     "fp8kv_decode_attn_window_bf16": (_c_i, _DECODE + [_c_f] + [_c_i] * 6 + [_c_vp, _c_sz] + [_c_i] * 3 + [_c_vp]),
     "fp8kv_decode_attn_blk": (_c_i, _DECODE + [_c_vp, _c_f] + [_c_i] * 6 + [_c_vp, _c_sz] + [_c_i] * 3 + [_c_vp]),

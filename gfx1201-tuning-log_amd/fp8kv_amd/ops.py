@@ -551,17 +551,21 @@ def _attention_args(q, k_cache, v_cache, out, starts, seq_lens, block_table, win
     return dev, bf16, (q.data_ptr(), q_stride, *caches, out.data_ptr(), o_stride, *seqs), (NS, HQ, HKV, D, PBLK), NB
 
 
+def decode_visible_splits(num_seqs: int, num_kv_heads: int, max_seq_len: int, window: int = 0, sinks: int = 0,
+                          bf16_kv: bool = False) -> int:
+    """The num_splits that ``decode_attention_window`` and ``decode_attention_blk`` take by themselves;
+    ``decode_scratch_bytes`` of it is what they need as scratch (max_seq_len 0: not known, with a window)."""
+    return _lib.load().fp8kv_decode_visible_splits(num_seqs, num_kv_heads, min(max_seq_len, 1 << 30), min(window, 1 << 30),
+                                                   min(sinks, 1 << 30), 1 if bf16_kv else 0)
+
+
 def _decode_visible(name, dev, lead, scales, sm_scale, geometry, q, seq_lens, window, sinks, num_splits, max_seq_len, scratch,
                     bf16_kv):
     NS, HQ, HKV, D, _ = geometry
     if num_splits is None:
-        if window > 0:
-            visible = window + sinks if max_seq_len is None else min(max_seq_len, window + sinks)
-        else:
-            if max_seq_len is None:
-                max_seq_len = int(seq_lens.max().item())
-            visible = max_seq_len
-        num_splits = decode_num_splits(NS, HKV, min(int(visible), 1 << 30), bf16_kv)
+        if max_seq_len is None and window == 0:
+            max_seq_len = int(seq_lens.max().item())
+        num_splits = decode_visible_splits(NS, HKV, max_seq_len or 0, window, sinks, bf16_kv)
     need = decode_scratch_bytes(NS, HQ, HKV, num_splits, D) if num_splits > 1 else 0
     if scratch is None:
         scratch = _call_scratch(need, q.device)

@@ -290,7 +290,10 @@ int fp8kv_prefill_attn_varlen_bf16(const void* q, int64_t q_row_stride,
  * fp8kv_prefill_attn_varlen, row i of sequence s at position seq_lens[s] - qlen_s + i.  Layouts, strides, geometry limits,
  * splits, scratch and max_seq_len as for fp8kv_decode_attn_ctx and fp8kv_prefill_attn_varlen (bf16: as for their bf16
  * forms); num_tokens is the number of queries of all sequences, for the launch plan alone (0: not known);
- * fp8kv_decode_num_splits is asked with the longest visible set, min(max_seq_len, window + sinks).
+ * fp8kv_decode_visible_splits is the library's choice of num_splits.
+ *   - Decode with num_splits > 1, 2 to 256 sequences and long contexts (max_seq_len and the window tell) may cut the
+ *     whole batch into equal parts instead of each sequence into num_splits: what a sequence's rounding is then
+ *     depends on the other lengths of the batch.  The scratch is that of num_splits either way.
  *   - Block-table entries of blocks without a visible key are never used, whatever they hold, so blocks that the
  *     window has left can be given back.
  *   - Rows that see nothing are zeros: seq_lens[s] <= 0, and rows of negative position (seq_lens[s] < qlen_s).
@@ -299,6 +302,10 @@ int fp8kv_prefill_attn_varlen_bf16(const void* q, int64_t q_row_stride,
  * Decode weighs V in two bf16 parts (error 2^-17 of a weight); prefill rounds the weights to bf16 and divides by
  * the sum of the rounded ones.
  * No counterpart in the reference, whose hook leaves such layers to stock vLLM (vllm-fp8kv/fp8kv_override.py:50-64). */
+/* num_splits of the decode calls below and of fp8kv_decode_attn_blk for a batch whose longest context is max_seq_len (0
+ * with a window: not known; >= 2^30: not known).  bf16: whether the caches are.  At most 256. */
+int fp8kv_decode_visible_splits(int num_seqs, int num_kv_heads, int max_seq_len, int window, int sinks, int bf16);
+
 int fp8kv_decode_attn_window(const void* q, int64_t q_row_stride,
                              const void* k_cache, const void* v_cache,
                              int64_t sk0, int64_t sk1, int64_t sk2,

@@ -1,5 +1,7 @@
 """Argument rejection of the append and visible-key attention calls, before any launch (no GPU; the pointers are
 never followed), and checks of their oracles."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -195,3 +197,29 @@ def test_oracle_agrees_with_the_whole_context_oracle_and_with_masked_softmax():
     a = visible.attention(*args[:6], (sc, 0), (sc, 1), c["sm_scale"], 6, 2)[0]
     b = visible.attention(*args[:6], 8.0, 1.0, c["sm_scale"], 6, 2)[0]
     assert torch.allclose(a, b, atol=1e-12)
+
+
+@pytest.mark.parametrize("ns,hkv,ctx,window,sinks,bf16,want", [
+    (32, 8, 2559, 0, 0, 0, 1), (32, 8, 2560, 0, 0, 0, 2), (32, 8, 100000, 2000, 559, 0, 1), (32, 8, 100000, 2000, 560, 0, 2),
+    (32, 8, 1279, 0, 0, 1, 1), (32, 8, 1280, 0, 0, 1, 2), (16, 4, 10239, 0, 0, 0, 4), (16, 4, 10240, 0, 0, 0, 5),
+    (24, 8, 2047, 0, 0, 0, 2), (24, 8, 2048, 0, 0, 0, 3), (128, 8, 2047, 0, 0, 0, 1), (128, 8, 2048, 0, 0, 0, 2),
+    (1, 4, 1 << 24, 0, 0, 0, 32), (257, 8, 1 << 24, 0, 0, 0, 1), (2, 1, 1 << 24, 0, 0, 0, 129), (2, 257, 1 << 24, 0, 0, 0, 1),
+    (2, 1, 1 << 30, 0, 0, 0, 32), (64, 8, 0, 0, 0, 0, 1), (64, 8, 0, 4096, 4, 0, 2), (64, 8, 0, 1 << 30, 4, 0, 1)])
+def test_decode_visible_split_plan(lib, ns, hkv, ctx, window, sinks, bf16, want):
+    """Both sides of the lines between splits of a sequence and equal parts of the batch; a count that a call takes."""
+    assert lib.fp8kv_decode_visible_splits(ns, hkv, ctx, window, sinks, bf16) == want
+    assert 1 <= want <= 256
+
+
+def test_prefill_visible_plan(lib):
+    out = (ctypes.c_int * 5)()
+    for hq, hkv in ((4, 4), (8, 4), (12, 4), (24, 4), (32, 4), (64, 4), (11, 1), (7, 7)):
+        for ns, longest, tokens in ((1, 1, 1), (1, 4096, 4096), (6, 900, 0), (40, 512, 3000), (200, 16, 3200), (65535, 1, 65535)):
+            for window, sinks in ((0, 0), (1024, 4), (16, 0)):
+                for bf16 in (0, 1):
+                    assert lib.fp8kv_prefill_visible_plan(hq, hkv, ns, longest, tokens, window, sinks, bf16, out) == 0
+                    sets, groups, blocks, paired, ranks = out
+                    assert sets in (2, 3) and groups in (2, 4, 8) and blocks >= 1 and ranks >= 1
+                    assert blocks * (hq // hkv) <= sets * groups                          # every row has a place
+                    assert (1 + paired) * ranks * blocks * 16 >= longest                  # and every token a workgroup
+    assert lib.fp8kv_prefill_visible_plan(3, 2, 1, 1, 1, 0, 0, 0, out) != 0

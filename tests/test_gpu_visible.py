@@ -131,6 +131,63 @@ def test_decode_many_sequences_and_long_context(kind):
     _check(_case(kind, [(20000, 1), (9000, 1)], 4, 1, 128, 6000, 50), "decode")
 
 
+PART_LENS = {
+    "ragged": [5000, 1, 0, 16, 17, 700, 0, 2300, 33],
+    "no_keys": [0, -3, 0, 0, 0],
+    "one_token": [1, 1, 1],
+    "long_last": [3, 0, 0, 9000],
+    "fewer_groups_than_parts": [100, 16, 40],
+    "one_group_more": [1040, 1024, 1024, 1023],
+    "many": [(37 * i) % 400 for i in range(200)],
+    "most": [(11 * i) % 60 for i in range(255)] + [700],
+    "too_many_to_share": [(11 * i) % 60 for i in range(257)],
+}
+LONG = 1 << 24                  # a longest context for which any batch is cut into parts
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lens", PART_LENS.values(), ids=PART_LENS.keys())
+def test_decode_parts(kind, lens):
+    """The walks of a batch in equal parts: boundaries inside sequences, parts of many sequences, sequences of many parts."""
+    lens = [(n - 1, 1) for n in lens]
+    for HQ, HKV, window, sinks in ((8, 2, 0, 0), (3, 1, 0, 0), (16, 16, 0, 0), (16, 16, 4000, 500), (2, 1, 4000, 500)):
+        if len(lens) > 50 and HKV > 2:
+            continue
+        c = _case(kind, lens, HQ, HKV, 32, window, sinks, seed=HKV)
+        splits = ops.decode_visible_splits(len(lens), HKV, LONG, window, sinks, kind == "bf16")
+        for n in {splits, 2, 3, 7}:
+            _check(c, "decode", num_splits=n, max_seq_len=LONG)
+
+
+def test_decode_parts_share_scratch():
+    """One scratch for calls of either shape and any lengths, in turn and replayed from a graph; same results every time."""
+    lens = [900, 1, 0, 3000, 64, 17]
+    c = _case("blk", [(n - 1, 1) for n in lens], 8, 2, 16, 0, 0, seed=5)
+    want, *bounds = _oracle(c)
+    d = {k: c[k].to(DEV) for k in ("q", "pool", "scales", "table", "starts", "seq_lens")}
+    k, v = workloads.engine_views(d["pool"], D)
+    splits = ops.decode_visible_splits(len(lens), 2, LONG)
+    scratch = ops.decode_scratch(ops.decode_scratch_bytes(len(lens), 8, 2, max(splits, 16), D), DEV)
+
+    def call(n, longest, lens=d["seq_lens"]):
+        out = torch.full_like(d["q"], 7.0)
+        return ops.decode_attention_blk(d["q"], k, v, out, d["starts"], lens, d["table"], d["scales"], c["sm"],
+                                        num_splits=n, max_seq_len=longest, scratch=scratch)
+    first = call(splits, LONG)
+    assert ((first.cpu().double() - want).abs() <= _tolerance(c, "decode", want, *bounds)).all()
+    moving = d["seq_lens"].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        replayed = call(splits, LONG, moving)
+    for i in range(4):
+        moving.copy_(torch.tensor([900 - 200 * i, 1, 0, 3000 - 7 * i, 64, 17 - i], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(replayed, call(splits, LONG, moving))
+        call(16, 3000)                                         # splits of each sequence over the same records
+        assert torch.equal(first, call(splits, LONG))
+
+
 PREFILL_LENS = {
     "short": [(0, 1), (0, 16), (0, 17), (0, 37), (0, 0), (5, 3)],
     "after_cached": [(200, 33), (5, 100), (31, 1), (64, 64)],
