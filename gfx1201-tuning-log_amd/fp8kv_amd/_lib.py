@@ -77,6 +77,9 @@ SIGNATURES: dict[str, tuple] = {
     "fp8kv_rope_append": (_c_i, _ROPE_APPEND + [_c_vp] * 3 + [_c_i] * 5 + [_c_i64, _c_vp]),
     "fp8kv_rope_append_bf16": (_c_i, _ROPE_APPEND + [_c_vp] + [_c_i] * 5 + [_c_i64, _c_vp]),
     "fp8kv_rope_append_blk": (_c_i, _ROPE_APPEND + [_c_vp] * 4 + [_c_i64] + [_c_i] * 7 + [_c_i64, _c_vp]),
+    # these calls with their arguments packed into 64-bit words (csrc/call_words.hip)
+    "fp8kv_call_entry": (_c_i, [ctypes.c_char_p]),
+    "fp8kv_call": (_c_i, [_c_i, ctypes.c_char_p, _c_i]),
     # layer epilogues (csrc/epilogues.hip, h4mv_silu_mul in csrc/h4mv.hip)
     "fp8kv_fused_add_rmsnorm": (_c_i, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_i, _c_i,
                                        _c_f, _c_i, _c_vp]),

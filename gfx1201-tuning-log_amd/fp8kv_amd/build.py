@@ -21,7 +21,8 @@ LIB_NAME = "libfp8kv_amd.so"
 LIB_PATH = os.path.join(PKG_ROOT, LIB_NAME)
 
 SOURCES = ["h4mv.hip", "h4mv_repack.hip", "decode_attn.hip", "prefill_attn.hip", "prefill_bf16kv.hip", "prefill_visible.hip",
-           "cache_write.hip", "rope_append.hip", "epilogues.hip", "w4a8_gemm.hip", "w4a8_slice.hip", "lm_head.hip"]
+           "cache_write.hip", "rope_append.hip", "epilogues.hip", "w4a8_gemm.hip", "w4a8_slice.hip", "lm_head.hip",
+           "call_words.hip"]
 # The benchmark's read-only reference launch (fp8kv_stream_read) is a measurement aid, not part of
 # the path: it is built into a library of its own that only bench.py loads.
 MEASURE_LIB_NAME = "libfp8kv_measure.so"

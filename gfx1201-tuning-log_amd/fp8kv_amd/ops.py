@@ -5,6 +5,10 @@ raises ``Fp8kvError`` if the library rejects the call.  Nothing here computes on
 """
 from __future__ import annotations
 
+import ctypes
+import functools
+import struct
+
 import torch
 
 from . import _lib
@@ -391,14 +395,24 @@ _E8M0 = torch.float8_e8m0fnu
 # The calls below run once per layer and step, like those above, and take a dozen tensors each.  Every property that is
 # read of a tensor costs about 0.1 us, so each is read once: shape and stride as whole tuples, the device as its number
 # (-1 on the CPU).
+@functools.lru_cache(maxsize=None)
+def _packed_entry(name: str) -> tuple:
+    """(fp8kv_call, number of the entry point, packer of its arguments, their count)."""
+    types = _lib.SIGNATURES[name][1]
+    lib = _lib.load()
+    return (lib.fp8kv_call, lib.fp8kv_call_entry(name.encode()),
+            struct.Struct("<" + "".join("f4x" if t is ctypes.c_float else "q" for t in types)).pack, len(types))
+
+
 def _launch(name: str, dev: int, *args) -> None:
-    """Entry point ``name`` on the current stream of device ``dev``, whichever device is current."""
-    fn = getattr(_lib.load(), name)
+    """Entry point ``name`` on the current stream of device ``dev``, whichever device is current (null pointers are 0)."""
+    call, entry, pack, count = _packed_entry(name)
     if dev == _current_device():
-        st = fn(*args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream)
+        st = call(entry, pack(*args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream),
+                  count)
     else:
         with torch.cuda.device(dev):
-            st = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            st = call(entry, pack(*args, torch.cuda.current_stream(dev).cuda_stream), count)
     if st != 0:
         _lib.check(name, st)
 
@@ -459,7 +473,7 @@ def _rope_args(q, key, value, positions, cos_sin, q_out, interleaved):
     vT, vH, vD, v_stride, v_dev = _heads(value, "value")
     if not (vT == T and vH == HKV and vD == D and v_dev == dev):
         raise ValueError("key and value must have the same shape and device")
-    HQ, q_args = 0, (None, 0, None, 0)
+    HQ, q_args = 0, (0, 0, 0, 0)
     if q is not None:
         qT, HQ, qD, q_stride, q_dev = _heads(q, "q")
         if q_out is None:
@@ -470,7 +484,7 @@ def _rope_args(q, key, value, positions, cos_sin, q_out, interleaved):
         q_args = (q.data_ptr(), q_stride, q_out.data_ptr(), o_stride)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    table = (None, None, 0, 0, 0, 0, 0)
+    table = (0, 0, 0, 0, 0, 0, 0)
     if cos_sin is not None:
         shape, stride, dtype = cos_sin.shape, cos_sin.stride(), cos_sin.dtype
         if not (len(shape) == 2 and (dtype is _F32 or dtype is _BF16) and stride[1] == 1 and cos_sin.get_device() == dev):
@@ -571,7 +585,7 @@ def _decode_visible(name, dev, lead, scales, sm_scale, geometry, q, seq_lens, wi
         scratch = _call_scratch(need, q.device)
     elif not (scratch.get_device() == dev and scratch.numel() * scratch.element_size() >= need):
         raise ValueError(f"scratch needs {need} bytes on device {dev}")
-    where, sbytes = (None, 0) if scratch is None else (scratch.data_ptr(), scratch.numel() * scratch.element_size())
+    where, sbytes = (0, 0) if scratch is None else (scratch.data_ptr(), scratch.numel() * scratch.element_size())
     _launch(name, dev, *lead, *scales, sm_scale, *geometry, num_splits, where, sbytes, window, sinks, max_seq_len or 0)
 
 

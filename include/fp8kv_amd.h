@@ -618,6 +618,15 @@ int fp8kv_rerank_exact(const void* E, int64_t e_row_stride, int V, const void* X
                        const int32_t* cand_idx, int C, int M, int H, float* out_val, int32_t* out_idx,
                        void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * The append and visible-key attention calls above (fp8kv_rope_append*, fp8kv_decode_attn_window*, _blk,
+ * fp8kv_prefill_attn_window*, _blk) with their arguments as 64-bit words, one each, in order: pointers and integers as
+ * they are, a float as its bits.  For callers to whom 35 arguments are more work than an array.
+ * fp8kv_call_entry: the call's number, or -1.  fp8kv_call: that call; FP8KV_ERR_ARG where `count` is not the number of
+ * its arguments or a word does not fit its argument. */
+int fp8kv_call_entry(const char* name);
+int fp8kv_call(int entry, const int64_t* words, int count);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,11 +1,13 @@
 """Argument rejection of the append and visible-key attention calls, before any launch (no GPU; the pointers are
 never followed), and checks of their oracles."""
 import ctypes
+import struct
 
 import numpy as np
 import pytest
 import torch
 
+from fp8kv_amd import _lib
 from oracle import attention, formats, rope_append, visible
 
 A = 0x10000
@@ -223,3 +225,42 @@ def test_prefill_visible_plan(lib):
                     assert blocks * (hq // hkv) <= sets * groups                          # every row has a place
                     assert (1 + paired) * ranks * blocks * 16 >= longest                  # and every token a workgroup
     assert lib.fp8kv_prefill_visible_plan(3, 2, 1, 1, 1, 0, 0, 0, out) != 0
+
+
+DECODE = [A, 4096, A, A + 128, 16384, 256, 4096, 16384, 256, 4096, A, 4096, A, A, A, 64]
+GEOMETRY = [2, 24, 4, 64, 16]                                # a head size that is refused
+BY_WORDS = {
+    "fp8kv_rope_append": (LEAD + [A, A, A] + TAIL, 0), "fp8kv_rope_append_bf16": (_lead(2) + [A] + TAIL, 0),
+    "fp8kv_rope_append_blk": (LEAD + [A, A, A, A, 64, 64, 1] + TAIL, 0),
+    "fp8kv_decode_attn_window": (DECODE + [A, A, 0.5] + GEOMETRY + [1, 0, 0, 64, 4, 100, 0], 2),
+    "fp8kv_decode_attn_window_bf16": (DECODE + [0.5] + GEOMETRY + [1, 0, 0, 64, 4, 100, 0], 2),
+    "fp8kv_decode_attn_blk": (DECODE + [A, 0.5] + GEOMETRY + [1, 0, 0, 64, 4, 100, 0], 2),
+    "fp8kv_prefill_attn_window": (DECODE + [A, A, 0.5] + GEOMETRY + [64, 4, 10, 20, 0], 2),
+    "fp8kv_prefill_attn_window_bf16": (DECODE + [0.5] + GEOMETRY + [64, 4, 10, 20, 0], 2),
+    "fp8kv_prefill_attn_blk": (DECODE + [A, 0.5] + GEOMETRY + [64, 4, 10, 20, 0], 2),
+}
+
+
+@pytest.mark.parametrize("name", BY_WORDS)
+def test_call_by_words(lib, name):
+    """The call's own answer, and a refusal where the words are too few or one is too large for its argument."""
+    args, code = BY_WORDS[name]
+    types = _lib.SIGNATURES[name][1]
+    assert len(types) == len(args)
+    entry = lib.fp8kv_call_entry(name.encode())
+    pack = struct.Struct("<" + "".join("f4x" if t is ctypes.c_float else "q" for t in types)).pack
+    args = [0 if x is None else x for x in args]
+    assert getattr(lib, name)(*args) == lib.fp8kv_call(entry, pack(*args), len(args)) == code
+    assert lib.fp8kv_call(entry, pack(*args), len(args) - 1) == 1
+    assert lib.fp8kv_call(entry, None, len(args)) == 1
+    for i, t in enumerate(types):
+        if t in (ctypes.c_int, ctypes.c_size_t):
+            wrong = [(1 << 32) + args[i], -(1 << 40)] if t is ctypes.c_int else [-1]
+            for x in wrong:
+                assert lib.fp8kv_call(entry, pack(*args[:i], x, *args[i + 1:]), len(args)) == 1, (i, x)
+
+
+def test_call_entries(lib):
+    assert sorted(lib.fp8kv_call_entry(n.encode()) for n in BY_WORDS) == list(range(len(BY_WORDS)))
+    assert lib.fp8kv_call_entry(b"fp8kv_cache_write") == lib.fp8kv_call_entry(None) == -1
+    assert lib.fp8kv_call(len(BY_WORDS), b"", 0) == lib.fp8kv_call(-1, b"", 0) == 1
