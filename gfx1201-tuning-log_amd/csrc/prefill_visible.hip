@@ -691,19 +691,18 @@ prefill_visible_kernel(VisibleParams P)
 }
 
 // ---- launch plan ----------------------------------------------------------------------------------
-// A workgroup takes nb token blocks of 16, whose nb * GQA row-sets fill the smallest shape that holds them.  More
-// blocks share the copies of their keys (which run at the L2's rate for one block of GQA 4 over bf16 caches), start and
-// end once, and leave fewer partial states to merge; fewer blocks split the keys over more waves, so the GPU is
-// full with fewer tokens.  The count follows from the time that a shape would take, in us:
-//   a workgroup   3 before and after its keys, 0.35 per key tile for the copies (0.7: bf16), and 1.5 (two row-sets a wave)
-//                 or 1.64 (three) per key tile and wave;
-//   the grid      its rounds of 256 workgroups: whole ones where the blocks cost alike (a window, pairs); half a round of
-//                 the mean for the end otherwise, and not less than the longest workgroup.
-// Where the context is not the window's, the host knows the queries only and takes them for it: a block sees their
-// number at most, half of it on average.  Measured, us with 1 / 2 / 4 blocks (GQA 6 and 4): 4096 after 1000, window
-// 1024, 109 / 89 / 73; 5 of 100..1500, bf16, window 512, 114 / 83 / 64; 2048, window 512 58 / 43 / 35; 300, window 100
-// 12.6 / 16.6 / 18.8; whole contexts, 6 of 37..900 after 200 63 / 52 / 64, 2048 after 2048 at GQA 4 155 / 129 / 141, at
-// GQA 6 103 / 113 / 194.
+// A workgroup takes nb token blocks of 16, whose nb * GQA row-sets fill a shape.  More blocks share the copies of their
+// keys, start and end once, and leave fewer partial states to merge; fewer blocks split the keys over more waves, so the
+// GPU is full with fewer tokens.  The shape follows from the time that each would take, in us, fitted to 100 batches
+// (1 to 16 sequences of 100..4000, GQA 4 to 10, either cache width) at every shape; the one taken is 1.7 % slower than
+// the best on average, 39 % at most:
+//   a workgroup   9.5, and per key tile 0.2 (bf16: 0.3) for its copies and 0.65 (two row-sets a wave) or 1.2 (three)
+//                 times the filled part of its eight waves, where a wave without rows still costs three quarters;
+//   the grid      its rounds of 256 workgroups and 0.4 for the end; where the blocks cost alike (a window, pairs) half
+//                 of a last round that is not full.  Not less than the longest workgroup.
+// The host knows the queries and not the context: 192 more keys than them stand for it, and a block of a whole context
+// sees 0.45 of its longest.  Measured, us with two / three row-sets of 2, 4 and 8 groups: GQA 4, 16 of 30..300, 71 / 60,
+// 49 / 51, 39 / 49; one of 4000, window 400, 83 / 85, 64 / 70, 55 / 64; 4 of 30..300 21 / 24, 17 / 22, 24 / 33.
 struct VisibleShape {
     int rs, ng;
 };
@@ -719,22 +718,26 @@ VisiblePlan plan_visible(bool b16, int gqa, int hkv, int num_seqs, int max_query
 {
     const double all = num_tokens > 0 ? num_tokens : (double)num_seqs * max_query_len;
     const bool limited = window > 0 && window < max_query_len;
+    const double longest = max_query_len + 192.0;
     VisiblePlan best{};
     double best_time = 1e300;
     for (const VisibleShape s : kVisibleShapes) {
         const int nb = s.rs * s.ng / gqa;
         if (nb < 1) continue;
-        const double tile = (b16 ? 0.7 : 0.35) + (s.rs == 2 ? 1.5 : 1.64) * s.ng / kSplitWaves;
-        const double most = 3 + tile / kBN * (limited ? (double)window + sinks + 16 * nb : (double)max_query_len);
-        const double mean = limited ? most : 3 + tile / kBN * max_query_len / 2;
-        const int n = (max_query_len + 16 * nb - 1) / (16 * nb);
-        const double blocks = num_seqs == 1 ? n : all / (16 * nb) + num_seqs / 2.0;
-        const double wgs = hkv * (blocks > num_seqs ? blocks : num_seqs);
+        const int block = 16 * nb, used = (nb * gqa + s.rs - 1) / s.rs;
+        const double tile = (b16 ? 0.3 : 0.2) + (s.rs == 2 ? 0.65 : 1.2) * (0.75 * s.ng + 0.25 * used) / kSplitWaves;
+        const double seen = (double)window + sinks + block;
+        const double most = 9.5 + tile / kBN * (limited && seen < longest ? seen : longest);
+        const double mean = limited ? most : 9.5 + tile / kBN * (0.45 * max_query_len + 192);
+        const int n = (max_query_len + block - 1) / block;
+        const double blocks = num_seqs == 1 ? n : all / block + num_seqs / 2.0;
         for (int paired = 0; paired < (limited ? 1 : 2); ++paired) {
-            const double x = wgs / (paired ? 2 : 1) / kSplitRoundWorkgroups;
-            double time = x <= 1 ? mean : limited || paired ? mean * ceil(x - 0.05) : mean * (x + 0.5);
-            if (paired) time *= 2;
-            else if (time < most) time = most;
+            // a sequence's last workgroup is half empty, or its only one
+            const double some = paired ? (num_seqs == 1 ? (n + 1) / 2 : (blocks + num_seqs / 2.0) / 2) : blocks;
+            const double x = hkv * (some > num_seqs ? some : num_seqs) / kSplitRoundWorkgroups;
+            const double one = paired ? 2 * mean : mean, least = paired ? 2 * mean : most;
+            double time = x <= 1 ? 0 : one * (limited || paired ? 0.5 * (x + 0.4 + ceil(x - 0.05)) : x + 0.4);
+            if (time < least) time = least;
             if (time < best_time) {
                 best_time = time;
                 best = VisiblePlan{s, nb, paired, paired ? (n + 1) / 2 : n};
