@@ -442,6 +442,16 @@ def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: int, D: int, allo
                                                 vs[0], vs[1], vs[2])
 
 
+def _scales(k_scale, v_scale, dev: int, like: torch.Tensor) -> tuple:
+    """The two scales of e4m3 caches as fp32 tensors on device dev, whose memory the call reads (so they are returned
+    and kept until it is queued)."""
+    if isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor):
+        if (k_scale.dtype is _F32 and v_scale.dtype is _F32 and k_scale.get_device() == dev and v_scale.get_device() == dev and
+                k_scale.numel() > 0 and v_scale.numel() > 0):
+            return k_scale, v_scale
+    return _scale_tensor(k_scale, like.device), _scale_tensor(v_scale, like.device)
+
+
 def _vector(t: torch.Tensor, name: str, dtype, n: int, dev: int) -> int:
     """Address of a contiguous vector of n elements."""
     shape = t.shape
@@ -520,7 +530,7 @@ def rope_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor, 
         return q_out
     if k_scale is None or v_scale is None:
         raise ValueError("e4m3 caches need k_scale and v_scale")
-    ks, vs = _scale_tensor(k_scale, key.device), _scale_tensor(v_scale, key.device)
+    ks, vs = _scales(k_scale, v_scale, dev, key)
     if T > 0:
         _launch("fp8kv_rope_append", dev, *rows, *caches, *table, slots, ks.data_ptr(), vs.data_ptr(), T, HQ, HKV, D, PBLK, NB)
     return q_out
@@ -573,19 +583,35 @@ def decode_visible_splits(num_seqs: int, num_kv_heads: int, max_seq_len: int, wi
                                                    min(sinks, 1 << 30), 1 if bf16_kv else 0)
 
 
+# What depends on sizes alone is asked for once per set of sizes: the bytes of scratch, and the plan with them.
+_visible_scratch_bytes = functools.lru_cache(maxsize=4096)(decode_scratch_bytes)
+
+
+@functools.lru_cache(maxsize=4096)
+def _visible_plan(NS, HQ, HKV, D, max_seq_len, window, sinks, bf16_kv):
+    splits = decode_visible_splits(NS, HKV, max_seq_len, window, sinks, bf16_kv)
+    return splits, decode_scratch_bytes(NS, HQ, HKV, splits, D)
+
+
 def _decode_visible(name, dev, lead, scales, sm_scale, geometry, q, seq_lens, window, sinks, num_splits, max_seq_len, scratch,
                     bf16_kv):
     NS, HQ, HKV, D, _ = geometry
     if num_splits is None:
         if max_seq_len is None and window == 0:
             max_seq_len = int(seq_lens.max().item())
-        num_splits = decode_visible_splits(NS, HKV, max_seq_len or 0, window, sinks, bf16_kv)
-    need = decode_scratch_bytes(NS, HQ, HKV, num_splits, D) if num_splits > 1 else 0
-    if scratch is None:
-        scratch = _call_scratch(need, q.device)
-    elif not (scratch.get_device() == dev and scratch.numel() * scratch.element_size() >= need):
-        raise ValueError(f"scratch needs {need} bytes on device {dev}")
-    where, sbytes = (0, 0) if scratch is None else (scratch.data_ptr(), scratch.numel() * scratch.element_size())
+        num_splits, need = _visible_plan(NS, HQ, HKV, D, max_seq_len or 0, window, sinks, bf16_kv)
+    else:
+        need = _visible_scratch_bytes(NS, HQ, HKV, num_splits, D) if num_splits > 1 else 0
+    where = sbytes = 0
+    if scratch is not None:
+        sbytes, where = scratch.numel() * scratch.element_size(), scratch.data_ptr()
+        if not (scratch.get_device() == dev and sbytes >= need):
+            raise ValueError(f"scratch needs {need} bytes on device {dev}")
+    elif need:
+        scratch = _scratch_cache.get(("cuda", dev))
+        if scratch is None or scratch.numel() < need:
+            scratch = _call_scratch(need, q.device)
+        sbytes, where = scratch.numel(), scratch.data_ptr()
     _launch(name, dev, *lead, *scales, sm_scale, *geometry, num_splits, where, sbytes, window, sinks, max_seq_len or 0)
 
 
@@ -605,7 +631,7 @@ def decode_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         return out
     name, scales = "fp8kv_decode_attn_window_bf16", ()
     if not bf16:
-        ks, vs = _scale_tensor(k_scale, q.device), _scale_tensor(v_scale, q.device)
+        ks, vs = _scales(k_scale, v_scale, dev, q)
         name, scales = "fp8kv_decode_attn_window", (ks.data_ptr(), vs.data_ptr())
     _decode_visible(name, dev, lead, scales, sm_scale, geometry, q, seq_lens, window, sinks, num_splits, max_seq_len, scratch,
                     bf16)
@@ -627,7 +653,7 @@ def prefill_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     if bf16:
         _launch("fp8kv_prefill_attn_window_bf16", dev, *lead, sm_scale, *geometry, window, sinks, max_query_len, q.shape[0])
     else:
-        ks, vs = _scale_tensor(k_scale, q.device), _scale_tensor(v_scale, q.device)
+        ks, vs = _scales(k_scale, v_scale, dev, q)
         _launch("fp8kv_prefill_attn_window", dev, *lead, ks.data_ptr(), vs.data_ptr(), sm_scale, *geometry, window, sinks,
                 max_query_len, q.shape[0])
     return out
