@@ -32,6 +32,8 @@
 #include "attn_common.h"
 #include "prefill_tiles.h"
 
+#include <type_traits>
+
 namespace fp8kv {
 namespace prefill_detail {
 
@@ -73,12 +75,25 @@ __device__ __forceinline__ float add_bf16x2(uint32_t w, float l)
 // What a weight may grow to before its row's reference moves, and how far above the row's max it moves then, in log2: a
 // row whose max then grows by less than the sum of the two is left alone, at weights between 2^-kLift and 2^kCeil.
 constexpr float kCeil = 256.f, kLift = 8.f;
+// References from here on are spaced so widely that the exact difference to one can leave a weight's range.
+constexpr float kFar = 0x1p28f;
 
-// New references and accumulators of RS row-sets after a weight past kCeil, from the tile's raw scores.
-template <int RS>
-__device__ __forceinline__ void lift_rows(const f32x4_t (&sc)[RS][2], float (&m_run)[RS], float (&l_run)[RS],
-                                          f32x4_t (&o)[RS][8], const float (&qkr)[RS])
+// The difference of a score, rounded, and a reference.
+__device__ __forceinline__ float rounded_difference(float x, float factor, float m)
 {
+#pragma clang fp contract(off)
+    const float s = x * factor;
+    return s - m;
+}
+
+// New references and accumulators of RS row-sets after a weight past kCeil, from the tile's raw scores.  Returns the
+// lanes where the reference of a row that has seen a key is past kFar.
+template <int RS>
+__device__ __forceinline__ uint64_t lift_rows(const f32x4_t (&sc)[RS][2], float (&m_run)[RS], float (&l_run)[RS],
+                                              f32x4_t (&o)[RS][8], const float (&qkr)[RS])
+{
+#pragma clang fp contract(off)                  // the max is rounded as the scores are
+    bool far = false;
 #pragma unroll
     for (int j = 0; j < RS; ++j) {
         float m = max3_raw(sc[j][0][0], sc[j][0][1], sc[j][0][2]);
@@ -91,7 +106,9 @@ __device__ __forceinline__ void lift_rows(const f32x4_t (&sc)[RS][2], float (&m_
 #pragma unroll
         for (int n = 0; n < 8; ++n) o[j][n] *= alpha;
         m_run[j] = m_new;
+        far |= fabsf(m_new) >= kFar && m_new > kMaxFloor;
     }
+    return __ballot(far);
 }
 
 // SC: block-scaled e4m3 caches.
@@ -344,6 +361,7 @@ prefill_visible_kernel(VisibleParams P)
 
         float m_run[RS], l_run[RS];
         f32x4_t o[RS][8];
+        uint64_t far = 0;                                          // lanes with a reference past kFar
 #pragma unroll
         for (int j = 0; j < RS; ++j) {
             m_run[j] = kMaxFloor;
@@ -498,17 +516,22 @@ prefill_visible_kernel(VisibleParams P)
                             }
                     }
                 }
-                // Weights of row-set j in bf16 (the P^T operand) and their sum.  The reference is a rounded product and the
-                // fused difference is not, so where scores are past 10^7 a row's largest weight is off by 2^+-(half a unit in
-                // the reference's last place): nothing to bf16 and its fp32 sums.
+                // Weights of row-set j in bf16 (the P^T operand) and their sum: of the exact difference of score and
+                // reference, which takes one instruction, or of the rounded product's, which is never above 2^-kLift for a
+                // reference that has moved.
                 u32x4_t pb[RS];
                 float ps[RS];
-                auto row_weights = [&](int j) {
+                auto row_weights = [&](int j, auto rounded) {
 #pragma unroll
                     for (int d = 0; d < 4; ++d) {
-                        const f32x4_t& x = sc[j][d >> 1];
-                        pb[j][d] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (d & 1)], qkr[j], -m_run[j])),
-                                               __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * (d & 1) + 1], qkr[j], -m_run[j])));
+                        float w[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float x = sc[j][d >> 1][2 * (d & 1) + e];
+                            w[e] = __builtin_amdgcn_exp2f(rounded ? rounded_difference(x, qkr[j], m_run[j])
+                                                                  : __builtin_fmaf(x, qkr[j], -m_run[j]));
+                        }
+                        pb[j][d] = pack_bf16x2(w[0], w[1]);
                     }
                     ps[j] = add_bf16x2(pb[j][3], add_bf16x2(pb[j][2], add_bf16x2(pb[j][1], add_bf16x2(pb[j][0], 0.f))));
                 };
@@ -518,13 +541,13 @@ prefill_visible_kernel(VisibleParams P)
                 bool over = false;
 #pragma unroll
                 for (int j = 0; j < RS; ++j) {
-                    row_weights(j);
+                    row_weights(j, std::false_type{});
                     over |= ps[j] > kCeil;
                 }
-                if (__any(over)) {
-                    lift_rows<RS>(sc, m_run, l_run, o, qkr);
+                if (__builtin_expect((__ballot(over) | far) != 0, 0)) {
+                    far = lift_rows<RS>(sc, m_run, l_run, o, qkr);
 #pragma unroll
-                    for (int j = 0; j < RS; ++j) row_weights(j);
+                    for (int j = 0; j < RS; ++j) row_weights(j, std::true_type{});
                 }
 #pragma unroll
                 for (int j = 0; j < RS; ++j) l_run[j] += ps[j];

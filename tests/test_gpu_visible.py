@@ -290,6 +290,34 @@ def test_large_scores_of_one_sign_and_zero_scale(form):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("form", ["decode", "prefill"])
+def test_huge_scores_pick_their_key(form, kind):
+    """Scores from 10^6 to 10^20: half a unit in the last place of one is more than a weight's whole range, and still
+    every row whose best key is best by more than the scores' error is that key's V."""
+    c = _case(kind, [(230, 1 if form == "decode" else 70), (31, 1 if form == "decode" else 40)], 6, 2, 16, 0, 0, seed=12)
+    for sm in (1e4, 1e6, 1e7, 3e7, 1e8, 1e10, -1e10, 1e18, -1e18):
+        c["sm"] = sm
+        want, _, reach = _oracle(c)
+        got = _run(c, form).double()
+        assert got.isfinite().all(), sm
+        k, _ = workloads.engine_views(c["pool"], D)
+        scale = (c["scales"], 0) if kind == "blk" else c["ks"]
+        clear = 0
+        for s in range(2):
+            a, b, length = int(c["starts"][s]), int(c["starts"][s + 1]), int(c["seq_lens"][s])
+            for i in range(a, b):
+                for h in range(2):
+                    keys = visible.rows(k, c["table"][s], torch.arange(length - (b - a) + i - a + 1), h, scale)
+                    best = (c["q"][i, 3 * h:3 * h + 3].double() @ keys.T * sm).sort(-1).values
+                    for r in range(3):
+                        row = 3 * h + r
+                        if best.shape[1] > 1 and best[r, -1] - best[r, -2] > 560 * 2.0 ** -24 * reach[i, row] + 20:
+                            clear += 1
+                            assert ((got[i, row] - want[i, row]).abs() <= 2.0 ** -8 * want[i, row].abs() + 1e-6).all(), (sm, i, row)
+        assert clear > 0.8 * 6 * int(c["starts"][-1])
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_strided_rows_and_untouched_output(kind):
     """q and out as slices of wider rows; only the rows of the sequences are written."""
     c = _case(kind, [(50, 20), (0, 9)], 4, 2, 16, 30, 4, seed=9)
