@@ -834,7 +834,7 @@ int prefill_visible(const void* q, int64_t q_row_stride, const void* k_cache, co
     P.cu_q = cu_seqlens_q;
     P.seq_lens = seq_lens;
     P.kv_scales = static_cast<const uint16_t*>(kv_scales);
-    P.window = window;
+    P.window = window < 1 << 30 ? window : 1 << 30;     // positions less a window stay within 32 bits
     P.sinks = sinks;
     return launch_visible(P, KIND == kBf16, num_seqs, max_query_len, num_tokens, reinterpret_cast<hipStream_t>(stream));
 }

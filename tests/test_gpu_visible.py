@@ -290,6 +290,14 @@ def test_large_scores_of_one_sign_and_zero_scale(form):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_largest_window_and_sinks(kind):
+    """Windows and sinks at the top of their range hide nothing, behind rows of negative position too."""
+    for window, sinks in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (1, 2 ** 31 - 1), (2 ** 30, 5)):
+        _check(_case(kind, [(-20, 70), (100, 33), (-5, 9)], 4, 2, 16, window, sinks, seed=13), "prefill")
+        _check(_case(kind, [(0, 1), (400, 1), (-1, 1), (70, 1)], 4, 2, 16, window, sinks, seed=14), "decode")
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("form", ["decode", "prefill"])
 def test_huge_scores_pick_their_key(form, kind):
     """Scores from 10^6 to 10^20: half a unit in the last place of one is more than a weight's whole range, and still
