@@ -800,6 +800,7 @@ inline int plan_parts(int ns, int hkv, int len, bool bf16)
 {
     const int64_t tokens = (int64_t)len * (bf16 ? 2 : 1), pairs = (int64_t)ns * hkv;
     if (ns < 2 || ns > kMaxShared || hkv > kCus || tokens < kLongWalk || len >= kUnknownContext) return 0;
+    if ((int64_t)ns * len >= (int64_t)1 << 34) return 0;          // the groups of a batch are counted in 32 bits
     const int64_t most = (int64_t)kCus * (pairs <= kCus && kCus % pairs == 0 ? kShareTokens : kShareTokens / 2);
     return pairs * tokens < most ? 0 : kCus / hkv;
 }

@@ -426,6 +426,14 @@ def _heads(t: torch.Tensor, name: str) -> tuple:
     return shape[0], shape[1], shape[2], stride[0] if shape[0] > 1 else shape[1] * shape[2], dev
 
 
+def _heads_like(t: torch.Tensor, name: str, shape: tuple, T: int, H: int, D: int, dev: int) -> int:
+    """Elements between the rows of a bf16 tensor of this shape and device whose heads are contiguous."""
+    stride = t.stride()
+    if not (t.shape == shape and t.dtype is _BF16 and t.get_device() == dev and stride[2] == 1 and (stride[1] == D or H == 1)):
+        raise ValueError(f"{name} must be a bf16 tensor {tuple(shape)} on device {dev} with contiguous heads")
+    return stride[0] if T > 1 else H * D
+
+
 def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: int, D: int, allow_bf16: bool) -> tuple:
     """(is bf16, NB, PBLK, HKV, addresses and strides as the C calls take them) of a cache's K and V views."""
     kd, vd = k_cache.dtype, v_cache.dtype
@@ -480,18 +488,16 @@ def _kv_scales(t: torch.Tensor, NB: int, PBLK: int, HKV: int, dev: int) -> int:
 def _rope_args(q, key, value, positions, cos_sin, q_out, interleaved):
     """Checks what the append calls share; (q_out, T, HQ, HKV, D, device, arguments of queries, keys, values, rotation)."""
     T, HKV, D, k_stride, dev = _heads(key, "key")
-    vT, vH, vD, v_stride, v_dev = _heads(value, "value")
-    if not (vT == T and vH == HKV and vD == D and v_dev == dev):
-        raise ValueError("key and value must have the same shape and device")
+    v_stride = _heads_like(value, "value", key.shape, T, HKV, D, dev)
     HQ, q_args = 0, (0, 0, 0, 0)
     if q is not None:
-        qT, HQ, qD, q_stride, q_dev = _heads(q, "q")
+        shape = q.shape
+        HQ = shape[1] if len(shape) == 3 else 0
         if q_out is None:
-            q_out = torch.empty((qT, HQ, qD), dtype=_BF16, device=q.device)
-        oT, oH, oD, o_stride, o_dev = _heads(q_out, "q_out")
-        if not (qT == oT == T and oH == HQ and qD == oD == D and q_dev == o_dev == dev):
-            raise ValueError("q and q_out must be [T, HQ, D] of key's T, D and device")
-        q_args = (q.data_ptr(), q_stride, q_out.data_ptr(), o_stride)
+            q_out = torch.empty(shape, dtype=_BF16, device=q.device)
+        shape = (T, HQ, D)
+        q_args = (q.data_ptr(), _heads_like(q, "q", shape, T, HQ, D, dev),
+                  q_out.data_ptr(), _heads_like(q_out, "q_out", shape, T, HQ, D, dev))
     elif q_out is not None:
         raise ValueError("q_out without q")
     table = (0, 0, 0, 0, 0, 0, 0)
@@ -596,9 +602,12 @@ def _visible_plan(NS, HQ, HKV, D, max_seq_len, window, sinks, bf16_kv):
 def _decode_visible(name, dev, lead, scales, sm_scale, geometry, q, seq_lens, window, sinks, num_splits, max_seq_len, scratch,
                     bf16_kv):
     NS, HQ, HKV, D, _ = geometry
+    window, sinks = int(window), int(sinks)
+    if max_seq_len is None and window == 0 and num_splits is None:
+        max_seq_len = seq_lens.max().item()
+    if max_seq_len is not None:
+        max_seq_len = int(max_seq_len)
     if num_splits is None:
-        if max_seq_len is None and window == 0:
-            max_seq_len = int(seq_lens.max().item())
         num_splits, need = _visible_plan(NS, HQ, HKV, D, max_seq_len or 0, window, sinks, bf16_kv)
     else:
         need = _visible_scratch_bytes(NS, HQ, HKV, num_splits, D) if num_splits > 1 else 0
