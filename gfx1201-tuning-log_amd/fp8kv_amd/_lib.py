@@ -6,10 +6,12 @@ Loading fails loudly: there is no CPU or Python fallback for any kernel.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import threading
 
-from .build import LIB_PATH, MEASURE_LIB_PATH
+from .build import CALLS_NAME, CALLS_PATH, LIB_PATH, MEASURE_LIB_PATH
 
 _c_vp = ctypes.c_void_p
 _c_i = ctypes.c_int
@@ -124,6 +126,7 @@ MEASURE_SIGNATURES: dict[str, tuple] = {
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 _measure: ctypes.CDLL | None = None
+_calls = None
 
 
 class Fp8kvError(RuntimeError):
@@ -181,6 +184,24 @@ def load_measure() -> ctypes.CDLL:
                 fn.argtypes = args
             _measure = lib
         return _measure
+
+
+def load_calls():
+    """Load (once) the torch extension module of the calls with many tensors, bound to the library."""
+    global _calls
+    lib = load()
+    with _lock:
+        if _calls is None:
+            if not os.path.exists(CALLS_PATH):
+                raise FileNotFoundError(f"{CALLS_PATH} is missing: build it with fp8kv_amd.build.build()")
+            loader = importlib.machinery.ExtensionFileLoader(CALLS_NAME, CALLS_PATH)
+            spec = importlib.util.spec_from_file_location(CALLS_NAME, CALLS_PATH, loader=loader)
+            module = importlib.util.module_from_spec(spec)
+            loader.exec_module(module)
+            module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in
+                          (lib.fp8kv_call, lib.fp8kv_decode_visible_splits, lib.fp8kv_decode_scratch_bytes)))
+            _calls = module
+        return _calls
 
 
 def check(fn_name: str, status: int) -> None:

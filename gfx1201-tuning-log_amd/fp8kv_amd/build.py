@@ -29,6 +29,12 @@ MEASURE_LIB_NAME = "libfp8kv_measure.so"
 MEASURE_LIB_PATH = os.path.join(PKG_ROOT, MEASURE_LIB_NAME)
 MEASURE_SOURCES = ["stream_read.hip"]
 
+# The torch side of the calls with many tensors (checks and argument packing, host code only): a Python
+# extension module, built against the torch that is installed.
+CALLS_NAME = "fp8kv_torch_calls"
+CALLS_PATH = os.path.join(PKG_ROOT, CALLS_NAME + ".so")
+CALLS_SOURCE = "torch_calls.cpp"
+
 # Packed-fp32 VALU forms are disabled for every HIP file built here (the compiler would otherwise
 # emit v_pk_{add,mul,fma}_f32 from ordinary float code).
 HIPCC_FLAGS = [
@@ -104,20 +110,42 @@ def _run(cmd: list[str], verbose: bool) -> str:
         print(" ".join(cmd), file=sys.stderr)
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({res.returncode}):\n{res.stderr[-6000:]}")
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({res.returncode}):\n{res.stderr[-6000:]}")
     return res.stderr
 
 
 def build(out: str = LIB_PATH, verbose: bool = False, jobs: int | None = None,
-          measure_out: str | None = MEASURE_LIB_PATH) -> str:
+          measure_out: str | None = MEASURE_LIB_PATH, calls_out: str | None = None) -> str:
     """Compile every source in SOURCES (one object each, in parallel) and link them into one
     shared library; atomic replace of ``out``.  Fails, leaving ``out`` untouched, when any kernel
     uses scratch memory (``resource_violations``).  Also builds the benchmark's measurement
-    library at ``measure_out`` (None: skipped)."""
+    library at ``measure_out`` (None: skipped) and the torch extension at ``calls_out`` (None: beside
+    the library if that is built in its place)."""
     path = _build_lib(SOURCES, out, verbose, jobs)
+    if calls_out is None and out == LIB_PATH:
+        calls_out = CALLS_PATH
+    if calls_out is not None:
+        build_calls(calls_out, verbose)
     if measure_out is not None:
         _build_lib(MEASURE_SOURCES, measure_out, verbose, jobs)
     return path
+
+
+def build_calls(out: str = CALLS_PATH, verbose: bool = False) -> str:
+    """Compile the torch extension module; atomic replace of ``out``."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    flags += [f"-isystem{d}" for d in cpp_extension.include_paths()] + [f"-I{sysconfig.get_paths()['include']}"]
+    libs = [f"-L{d}" for d in cpp_extension.library_paths()] + ["-ltorch_python", "-ltorch_cpu", "-lc10"]
+    with tempfile.TemporaryDirectory(prefix=".fp8kv_amd_build_", dir=os.path.dirname(out)) as tmpdir:
+        tmp = os.path.join(tmpdir, os.path.basename(out))
+        _run([os.environ.get("CXX", "g++"), *flags, os.path.join(CSRC, CALLS_SOURCE), "-o", tmp, *libs], verbose)
+        os.replace(tmp, out)
+    return out
 
 
 def _build_lib(sources: list[str], out: str, verbose: bool, jobs: int | None) -> str:

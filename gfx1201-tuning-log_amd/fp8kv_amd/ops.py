@@ -5,9 +5,7 @@ raises ``Fp8kvError`` if the library rejects the call.  Nothing here computes on
 """
 from __future__ import annotations
 
-import ctypes
 import functools
-import struct
 
 import torch
 
@@ -387,130 +385,33 @@ def rope_table(num_positions: int, rotary_dim: int, device, base: float = 10000.
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-_BF16, _E4M3, _U8, _I32, _I64, _F32 = (torch.bfloat16, torch.float8_e4m3fn, torch.uint8, torch.int32, torch.int64,
-                                       torch.float32)
-_E8M0 = torch.float8_e8m0fnu
 
 
-# The calls below run once per layer and step, like those above, and take a dozen tensors each.  Every property that is
-# read of a tensor costs about 0.1 us, so each is read once: shape and stride as whole tuples, the device as its number
-# (-1 on the CPU).
+# The calls below take a dozen tensors each and run once per layer and step, so their checks, and the packing of their
+# arguments, are native (csrc/torch_calls.cpp); here are defaults, the stream and the memory they need.
 @functools.lru_cache(maxsize=None)
-def _packed_entry(name: str) -> tuple:
-    """(fp8kv_call, number of the entry point, packer of its arguments, their count)."""
-    types = _lib.SIGNATURES[name][1]
+def _native(method: str, *names: str) -> tuple:
+    """(the native call, the numbers of the entry points that it chooses from)."""
     lib = _lib.load()
-    return (lib.fp8kv_call, lib.fp8kv_call_entry(name.encode()),
-            struct.Struct("<" + "".join("f4x" if t is ctypes.c_float else "q" for t in types)).pack, len(types))
+    return getattr(_lib.load_calls(), method), *(lib.fp8kv_call_entry(n.encode()) for n in names)
 
 
-def _launch(name: str, dev: int, *args) -> None:
-    """Entry point ``name`` on the current stream of device ``dev``, whichever device is current (null pointers are 0)."""
-    call, entry, pack, count = _packed_entry(name)
+def _run(native: tuple, dev: int, *args) -> int:
+    """The native call on the current stream of device ``dev``, whichever device is current."""
+    if dev < 0:                                   # a CPU tensor, which the call refuses
+        return native[0](*native[1:], 0, *args)
     if dev == _current_device():
-        st = call(entry, pack(*args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream),
-                  count)
-    else:
-        with torch.cuda.device(dev):
-            st = call(entry, pack(*args, torch.cuda.current_stream(dev).cuda_stream), count)
-    if st != 0:
-        _lib.check(name, st)
+        return native[0](*native[1:], _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream,
+                         *args)
+    with torch.cuda.device(dev):
+        return native[0](*native[1:], torch.cuda.current_stream(dev).cuda_stream, *args)
 
 
-def _heads(t: torch.Tensor, name: str) -> tuple:
-    """(T, H, D, elements between the rows, device) of a bf16 [T, H, D] tensor whose heads are contiguous.  A
-    single row's stride says nothing and is replaced."""
-    shape, stride, dev = t.shape, t.stride(), t.get_device()
-    if not (len(shape) == 3 and t.dtype is _BF16 and dev >= 0 and stride[2] == 1 and (stride[1] == shape[2] or shape[1] == 1)):
-        raise ValueError(f"{name} must be a bf16 device tensor [T, heads, D] with contiguous heads")
-    return shape[0], shape[1], shape[2], stride[0] if shape[0] > 1 else shape[1] * shape[2], dev
-
-
-def _heads_like(t: torch.Tensor, name: str, shape: tuple, T: int, H: int, D: int, dev: int) -> int:
-    """Elements between the rows of a bf16 tensor of this shape and device whose heads are contiguous."""
-    stride = t.stride()
-    if not (t.shape == shape and t.dtype is _BF16 and t.get_device() == dev and stride[2] == 1 and (stride[1] == D or H == 1)):
-        raise ValueError(f"{name} must be a bf16 tensor {tuple(shape)} on device {dev} with contiguous heads")
-    return stride[0] if T > 1 else H * D
-
-
-def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: int, D: int, allow_bf16: bool) -> tuple:
-    """(is bf16, NB, PBLK, HKV, addresses and strides as the C calls take them) of a cache's K and V views."""
-    kd, vd = k_cache.dtype, v_cache.dtype
-    bf16 = kd is _BF16 and vd is _BF16
-    if not (bf16 and allow_bf16) and not ((kd is _E4M3 or kd is _U8) and (vd is _E4M3 or vd is _U8)):
-        raise ValueError("caches must both be e4m3 (float8_e4m3fn or raw uint8)" + (" or both bf16" if allow_bf16 else ""))
-    ks, vs = k_cache.stride(), v_cache.stride()
-    shape = k_cache.shape
-    if not (len(shape) == 4 and shape == v_cache.shape and shape[3] == D and ks[3] == 1 and vs[3] == 1):
-        raise ValueError("caches must be [NB, PBLK, HKV, D] of one shape, contiguous along the head size that q and key have")
-    if not (k_cache.get_device() == dev and v_cache.get_device() == dev):
-        raise ValueError("tensors on different devices")
-    return bf16, shape[0], shape[1], shape[2], (k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2],
-                                                vs[0], vs[1], vs[2])
-
-
-def _scales(k_scale, v_scale, dev: int, like: torch.Tensor) -> tuple:
-    """The two scales of e4m3 caches as fp32 tensors on device dev, whose memory the call reads (so they are returned
-    and kept until it is queued)."""
-    if isinstance(k_scale, torch.Tensor) and isinstance(v_scale, torch.Tensor):
-        if (k_scale.dtype is _F32 and v_scale.dtype is _F32 and k_scale.get_device() == dev and v_scale.get_device() == dev and
-                k_scale.numel() > 0 and v_scale.numel() > 0):
-            return k_scale, v_scale
-    return _scale_tensor(k_scale, like.device), _scale_tensor(v_scale, like.device)
-
-
-def _vector(t: torch.Tensor, name: str, dtype, n: int, dev: int) -> int:
-    """Address of a contiguous vector of n elements."""
-    shape = t.shape
-    if not (t.dtype is dtype and len(shape) == 1 and shape[0] == n and t.is_contiguous() and t.get_device() == dev):
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor [{n}] on device {dev}")
-    return t.data_ptr()
-
-
-def _sequences(starts: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, dev: int) -> tuple:
-    """(NS, max_blocks, addresses and stride) of the sequences' metadata."""
-    shape, stride = block_table.shape, block_table.stride()
-    if not (len(shape) == 2 and block_table.dtype is _I32 and (stride[1] == 1 or shape[1] <= 1) and
-            block_table.get_device() == dev):
-        raise ValueError(f"block_table must be an int32 tensor [NS, max_blocks] on device {dev}, rows contiguous")
-    return shape[0], shape[1], (_vector(starts, "query_start_loc", _I32, shape[0] + 1, dev),
-                                _vector(seq_lens, "seq_lens", _I32, shape[0], dev), block_table.data_ptr(), stride[0])
-
-
-def _kv_scales(t: torch.Tensor, NB: int, PBLK: int, HKV: int, dev: int) -> int:
-    if not ((t.dtype is _U8 or t.dtype is _E8M0) and t.shape == (NB, PBLK // 16, HKV, 2) and t.is_contiguous() and
-            t.get_device() == dev):
-        raise ValueError(f"kv_scales must be contiguous uint8 (e8m0) [{NB}, {PBLK // 16}, {HKV}, 2] on device {dev}")
-    return t.data_ptr()
-
-
-def _rope_args(q, key, value, positions, cos_sin, q_out, interleaved):
-    """Checks what the append calls share; (q_out, T, HQ, HKV, D, device, arguments of queries, keys, values, rotation)."""
-    T, HKV, D, k_stride, dev = _heads(key, "key")
-    v_stride = _heads_like(value, "value", key.shape, T, HKV, D, dev)
-    HQ, q_args = 0, (0, 0, 0, 0)
-    if q is not None:
-        shape = q.shape
-        HQ = shape[1] if len(shape) == 3 else 0
-        if q_out is None:
-            q_out = torch.empty(shape, dtype=_BF16, device=q.device)
-        shape = (T, HQ, D)
-        q_args = (q.data_ptr(), _heads_like(q, "q", shape, T, HQ, D, dev),
-                  q_out.data_ptr(), _heads_like(q_out, "q_out", shape, T, HQ, D, dev))
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    table = (0, 0, 0, 0, 0, 0, 0)
-    if cos_sin is not None:
-        shape, stride, dtype = cos_sin.shape, cos_sin.stride(), cos_sin.dtype
-        if not (len(shape) == 2 and (dtype is _F32 or dtype is _BF16) and stride[1] == 1 and cos_sin.get_device() == dev):
-            raise ValueError("cos_sin must be fp32 or bf16 [positions, rotary_dim] on key's device")
-        if positions is None:
-            raise ValueError("cos_sin without positions")
-        table = (_vector(positions, "positions", _I64, T, dev), cos_sin.data_ptr(),
-                 stride[0] if shape[0] > 1 else shape[1], 1 if dtype is _BF16 else 0, shape[0], shape[1],
-                 1 if interleaved else 0)
-    return q_out, T, HQ, HKV, D, dev, (*q_args, key.data_ptr(), k_stride, value.data_ptr(), v_stride), table
+def _scale_pair(k_scale, v_scale, cache: torch.Tensor) -> tuple:
+    """The scales of e4m3 caches as tensors (a number becomes one on the caches' device)."""
+    if type(k_scale) is torch.Tensor and type(v_scale) is torch.Tensor or cache.dtype is torch.bfloat16:
+        return k_scale, v_scale
+    return tuple(x if x is None else _scale_tensor(x, cache.device) for x in (k_scale, v_scale))
 
 
 def rope_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor,
@@ -525,20 +426,13 @@ def rope_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor, 
     (``rope_table``); the first R elements of a head are rotated, paired in halves or, ``interleaved``,
     adjacent.  A position outside the table gives NaN.  ``cos_sin=None``: no rotation; ``q=None``: keys and
     values only.  fp32 arithmetic, rounded once (fp8kv_rope_append)."""
-    q_out, T, HQ, HKV, D, dev, rows, table = _rope_args(q, key, value, positions, cos_sin, q_out, interleaved)
-    bf16_kv, NB, PBLK, cH, caches = _caches(k_cache, v_cache, dev, D, True)
-    if cH != HKV:
-        raise ValueError("caches must be [NB, PBLK, HKV, D] matching key")
-    slots = _vector(slot_mapping, "slot_mapping", _I64, T, dev)
-    if bf16_kv:
-        if T > 0:
-            _launch("fp8kv_rope_append_bf16", dev, *rows, *caches, *table, slots, T, HQ, HKV, D, PBLK, NB)
-        return q_out
-    if k_scale is None or v_scale is None:
-        raise ValueError("e4m3 caches need k_scale and v_scale")
-    ks, vs = _scales(k_scale, v_scale, dev, key)
-    if T > 0:
-        _launch("fp8kv_rope_append", dev, *rows, *caches, *table, slots, ks.data_ptr(), vs.data_ptr(), T, HQ, HKV, D, PBLK, NB)
+    if q is not None and q_out is None:
+        q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    k_scale, v_scale = _scale_pair(k_scale, v_scale, k_cache)
+    st = _run(_native("rope_append", "fp8kv_rope_append", "fp8kv_rope_append_bf16"), key.get_device(), q, key, value, k_cache,
+              v_cache, positions, cos_sin, q_out, interleaved, slot_mapping, k_scale, v_scale)
+    if st:
+        _lib.check("fp8kv_rope_append", st)
     return q_out
 
 
@@ -555,31 +449,16 @@ def rope_append_blk(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tens
     row s (int32 device tensors, the metadata of the attention calls).  A group of 16 that also holds
     earlier tokens keeps its scale unless the new ones need a larger one; then the old codes are re-rounded.
     Rows of q_out behind the last sequence are left as they were (fp8kv_rope_append_blk)."""
-    q_out, T, HQ, HKV, D, dev, rows, table = _rope_args(q, key, value, positions, cos_sin, q_out, interleaved)
-    _, NB, PBLK, cH, caches = _caches(k_cache, v_cache, dev, D, False)
-    if cH != HKV:
-        raise ValueError("caches must be [NB, PBLK, HKV, D] matching key")
-    scales = _kv_scales(kv_scales, NB, PBLK, HKV, dev)
-    NS, max_blocks, seqs = _sequences(query_start_loc, seq_lens, block_table, dev)
-    if T > 0 and NS > 0:
-        _launch("fp8kv_rope_append_blk", dev, *rows, *caches, *table, scales, *seqs, max_blocks, NS, T, HQ, HKV, D, PBLK, NB)
+    if q is not None and q_out is None:
+        q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    st = _run(_native("rope_append_blk", "fp8kv_rope_append_blk"), key.get_device(), q, key, value, k_cache, v_cache, positions,
+              cos_sin, q_out, interleaved, kv_scales, query_start_loc, seq_lens, block_table)
+    if st:
+        _lib.check("fp8kv_rope_append_blk", st)
     return q_out
 
 
 # ------------------------------------------------------------------------------ attention over visible keys
-
-def _attention_args(q, k_cache, v_cache, out, starts, seq_lens, block_table, window, sinks, allow_bf16):
-    """Checks what the calls below share; (device, is bf16, leading arguments, trailing geometry) of the C calls."""
-    _, HQ, D, q_stride, dev = _heads(q, "q")
-    _, oH, oD, o_stride, o_dev = _heads(out, "out")
-    if not (oH == HQ and oD == D and o_dev == dev):
-        raise ValueError("out must be [T, HQ, D] of q's heads and device")
-    bf16, NB, PBLK, HKV, caches = _caches(k_cache, v_cache, dev, D, allow_bf16)
-    NS, _, seqs = _sequences(starts, seq_lens, block_table, dev)
-    if window < 0 or sinks < 0:
-        raise ValueError("window and sinks must not be negative")
-    return dev, bf16, (q.data_ptr(), q_stride, *caches, out.data_ptr(), o_stride, *seqs), (NS, HQ, HKV, D, PBLK), NB
-
 
 def decode_visible_splits(num_seqs: int, num_kv_heads: int, max_seq_len: int, window: int = 0, sinks: int = 0,
                           bf16_kv: bool = False) -> int:
@@ -589,39 +468,24 @@ def decode_visible_splits(num_seqs: int, num_kv_heads: int, max_seq_len: int, wi
                                                    min(sinks, 1 << 30), 1 if bf16_kv else 0)
 
 
-# What depends on sizes alone is asked for once per set of sizes: the bytes of scratch, and the plan with them.
-_visible_scratch_bytes = functools.lru_cache(maxsize=4096)(decode_scratch_bytes)
+def _longest_query(starts: torch.Tensor) -> int:
+    return int((starts[1:] - starts[:-1]).max().item()) if starts.numel() > 1 else 0
 
 
-@functools.lru_cache(maxsize=4096)
-def _visible_plan(NS, HQ, HKV, D, max_seq_len, window, sinks, bf16_kv):
-    splits = decode_visible_splits(NS, HKV, max_seq_len, window, sinks, bf16_kv)
-    return splits, decode_scratch_bytes(NS, HQ, HKV, splits, D)
-
-
-def _decode_visible(name, dev, lead, scales, sm_scale, geometry, q, seq_lens, window, sinks, num_splits, max_seq_len, scratch,
-                    bf16_kv):
-    NS, HQ, HKV, D, _ = geometry
-    window, sinks = int(window), int(sinks)
-    if max_seq_len is None and window == 0 and num_splits is None:
-        max_seq_len = seq_lens.max().item()
-    if max_seq_len is not None:
-        max_seq_len = int(max_seq_len)
-    if num_splits is None:
-        num_splits, need = _visible_plan(NS, HQ, HKV, D, max_seq_len or 0, window, sinks, bf16_kv)
-    else:
-        need = _visible_scratch_bytes(NS, HQ, HKV, num_splits, D) if num_splits > 1 else 0
-    where = sbytes = 0
-    if scratch is not None:
-        sbytes, where = scratch.numel() * scratch.element_size(), scratch.data_ptr()
-        if not (scratch.get_device() == dev and sbytes >= need):
-            raise ValueError(f"scratch needs {need} bytes on device {dev}")
-    elif need:
-        scratch = _scratch_cache.get(("cuda", dev))
-        if scratch is None or scratch.numel() < need:
-            scratch = _call_scratch(need, q.device)
-        sbytes, where = scratch.numel(), scratch.data_ptr()
-    _launch(name, dev, *lead, *scales, sm_scale, *geometry, num_splits, where, sbytes, window, sinks, max_seq_len or 0)
+def _decode(native, name, q, k_cache, v_cache, out, starts, seq_lens, block_table, scales, sm_scale, window, sinks, num_splits,
+            max_seq_len, scratch):
+    if max_seq_len is None:
+        if window == 0 and num_splits is None and seq_lens.numel() > 0:
+            max_seq_len = int(seq_lens.max().item())
+        else:
+            max_seq_len = 0
+    dev = q.get_device()
+    args = (q, k_cache, v_cache, out, starts, seq_lens, block_table, *scales, sm_scale, window, sinks, num_splits, max_seq_len)
+    st = _run(native, dev, *args, _scratch_cache.get(("cuda", dev)) if scratch is None else scratch, scratch is not None)
+    if st < 0:                                    # the bytes of scratch it needs
+        st = _run(native, dev, *args, _call_scratch(-st, q.device), True)
+    if st:
+        _lib.check(name, st)
 
 
 def decode_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor,
@@ -634,16 +498,9 @@ def decode_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
     Only the visible keys are read; block-table entries of blocks that hold none may be anything.  A window bounds
     the work, so ``max_seq_len`` is needed only without one (and then read from ``seq_lens``, which synchronises)."""
-    dev, bf16, lead, geometry, _ = _attention_args(q, k_cache, v_cache, out, query_start_loc, seq_lens, block_table, window,
-                                                   sinks, True)
-    if geometry[0] == 0:
-        return out
-    name, scales = "fp8kv_decode_attn_window_bf16", ()
-    if not bf16:
-        ks, vs = _scales(k_scale, v_scale, dev, q)
-        name, scales = "fp8kv_decode_attn_window", (ks.data_ptr(), vs.data_ptr())
-    _decode_visible(name, dev, lead, scales, sm_scale, geometry, q, seq_lens, window, sinks, num_splits, max_seq_len, scratch,
-                    bf16)
+    _decode(_native("decode", "fp8kv_decode_attn_window", "fp8kv_decode_attn_window_bf16"), "fp8kv_decode_attn_window", q, k_cache,
+            v_cache, out, query_start_loc, seq_lens, block_table, _scale_pair(k_scale, v_scale, k_cache), sm_scale, window, sinks,
+            num_splits, max_seq_len, scratch)
     return out
 
 
@@ -653,18 +510,12 @@ def prefill_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
                              max_query_len: int | None = None) -> torch.Tensor:
     """``prefill_attention_varlen`` where the query at position p sees the keys t <= p with t > p - window
     or t < sinks (window 0: all t <= p).  Caches e4m3 with per-tensor scales, or bf16."""
-    dev, bf16, lead, geometry, _ = _attention_args(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, window,
-                                                   sinks, True)
-    if geometry[0] == 0 or q.shape[0] == 0:
-        return out
-    if max_query_len is None:
-        max_query_len = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item())
-    if bf16:
-        _launch("fp8kv_prefill_attn_window_bf16", dev, *lead, sm_scale, *geometry, window, sinks, max_query_len, q.shape[0])
-    else:
-        ks, vs = _scales(k_scale, v_scale, dev, q)
-        _launch("fp8kv_prefill_attn_window", dev, *lead, ks.data_ptr(), vs.data_ptr(), sm_scale, *geometry, window, sinks,
-                max_query_len, q.shape[0])
+    k_scale, v_scale = _scale_pair(k_scale, v_scale, k_cache)
+    st = _run(_native("prefill", "fp8kv_prefill_attn_window", "fp8kv_prefill_attn_window_bf16"), q.get_device(), q, k_cache, v_cache,
+              out, cu_seqlens_q, seq_lens, block_table, k_scale, v_scale, sm_scale, window, sinks,
+              _longest_query(cu_seqlens_q) if max_query_len is None else max_query_len)
+    if st:
+        _lib.check("fp8kv_prefill_attn_window", st)
     return out
 
 
@@ -675,12 +526,8 @@ def decode_attention_blk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
                          scratch: torch.Tensor | None = None) -> torch.Tensor:
     """``decode_attention`` over the block-scaled e4m3 cache that ``rope_append_blk`` writes (``kv_scales`` uint8
     [NB, PBLK / 16, HKV, 2]), with ``window`` and ``sinks`` as in ``decode_attention_window``."""
-    dev, _, lead, geometry, NB = _attention_args(q, k_cache, v_cache, out, query_start_loc, seq_lens, block_table, window,
-                                                 sinks, False)
-    scales = _kv_scales(kv_scales, NB, geometry[4], geometry[2], dev)
-    if geometry[0] > 0:
-        _decode_visible("fp8kv_decode_attn_blk", dev, lead, (scales,), sm_scale, geometry, q, seq_lens, window, sinks,
-                        num_splits, max_seq_len, scratch, False)
+    _decode(_native("decode_blk", "fp8kv_decode_attn_blk", "fp8kv_decode_attn_blk"), "fp8kv_decode_attn_blk", q, k_cache, v_cache,
+            out, query_start_loc, seq_lens, block_table, (kv_scales, None), sm_scale, window, sinks, num_splits, max_seq_len, scratch)
     return out
 
 
@@ -690,14 +537,11 @@ def prefill_attention_blk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
                           max_query_len: int | None = None) -> torch.Tensor:
     """``prefill_attention_varlen`` over the block-scaled e4m3 cache that ``rope_append_blk`` writes, with ``window``
     and ``sinks`` as in ``prefill_attention_window``."""
-    dev, _, lead, geometry, NB = _attention_args(q, k_cache, v_cache, out, cu_seqlens_q, seq_lens, block_table, window,
-                                                 sinks, False)
-    scales = _kv_scales(kv_scales, NB, geometry[4], geometry[2], dev)
-    if geometry[0] == 0 or q.shape[0] == 0:
-        return out
-    if max_query_len is None:
-        max_query_len = int((cu_seqlens_q[1:] - cu_seqlens_q[:-1]).max().item())
-    _launch("fp8kv_prefill_attn_blk", dev, *lead, scales, sm_scale, *geometry, window, sinks, max_query_len, q.shape[0])
+    st = _run(_native("prefill_blk", "fp8kv_prefill_attn_blk", "fp8kv_prefill_attn_blk"), q.get_device(), q, k_cache, v_cache, out,
+              cu_seqlens_q, seq_lens, block_table, kv_scales, None, sm_scale, window, sinks,
+              _longest_query(cu_seqlens_q) if max_query_len is None else max_query_len)
+    if st:
+        _lib.check("fp8kv_prefill_attn_blk", st)
     return out
 
 

@@ -264,3 +264,25 @@ def test_call_entries(lib):
     assert sorted(lib.fp8kv_call_entry(n.encode()) for n in BY_WORDS) == list(range(len(BY_WORDS)))
     assert lib.fp8kv_call_entry(b"fp8kv_cache_write") == lib.fp8kv_call_entry(None) == -1
     assert lib.fp8kv_call(len(BY_WORDS), b"", 0) == lib.fp8kv_call(-1, b"", 0) == 1
+
+
+def test_wrappers_refuse_host_tensors():
+    """The checks of the torch wrappers are native: tensors that are not on a device never reach the library."""
+    from fp8kv_amd import ops
+    x = torch.zeros(2, 4, 128, dtype=torch.bfloat16)
+    kc, slots, i32 = torch.zeros(1, 16, 4, 128, dtype=torch.uint8), torch.zeros(2, dtype=torch.int64), torch.zeros(2, dtype=torch.int32)
+    one, scales, table = torch.ones(1), torch.full((1, 1, 4, 2), 127, dtype=torch.uint8), torch.zeros(1, 1, dtype=torch.int32)
+    for call in (lambda: ops.rope_append(x, x, x, kc, kc, None, None, slots, one, one),
+                 lambda: ops.rope_append_blk(x, x, x, kc, kc, scales, None, None, i32, i32[:1], table),
+                 lambda: ops.decode_attention_window(x, kc, kc, x, i32, i32[:1], table, one, one, 0.1, 4),
+                 lambda: ops.decode_attention_blk(x, kc, kc, x, i32, i32[:1], table, scales, 0.1),
+                 lambda: ops.prefill_attention_window(x, kc, kc, x, i32, i32[:1], table, one, one, 0.1, 4),
+                 lambda: ops.prefill_attention_blk(x, kc, kc, x, i32, i32[:1], table, scales, 0.1, max_query_len=2)):
+        with pytest.raises(ValueError, match="device tensor"):
+            call()
+    native = _lib.load_calls()
+    for name in ("rope_append", "rope_append_blk", "decode", "decode_blk", "prefill", "prefill_blk"):
+        with pytest.raises(TypeError, match="arguments"):
+            getattr(native, name)(x, x)
+    with pytest.raises(ValueError, match="tensor"):
+        native.rope_append(0, 1, 0, None, 3, x, kc, kc, None, None, None, False, slots, one, one)
