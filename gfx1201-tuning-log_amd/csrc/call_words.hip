@@ -1,7 +1,7 @@
 // fp8kv_call: entry points with many arguments, called with all of them in one array of 64-bit words.
 //
-// For an interpreter, which converts 35 arguments one by one: ctypes 4.7 to 5.0 us a call with its launch, struct.pack
-// and a call with a pointer 3.7 to 3.9, and a decode step makes several such calls per layer.
+// For bindings, which convert 35 arguments one by one otherwise (ctypes: 4.7 to 5.0 us a call with its launch, an array
+// of words 3.7 to 3.9), and check here that every word fits its argument.
 #include "fp8kv_common.h"
 #include "fp8kv_status.h"
 

@@ -285,16 +285,17 @@ int64_t decode(PyObject* const* a, bool blk)
     const int64_t longest = integer(a[16]), window = integer(a[13]), sinks = integer(a[14]);
     const int64_t splits = a[15] != Py_None ? integer(a[15])
                                             : g_splits(size(r.NS), size(r.c.HKV), size(longest), size(window), size(sinks), r.c.bf16);
-    const int64_t need = splits > 1 ? (int64_t)g_scratch_bytes(size(r.NS), size(r.q.H), size(r.c.HKV), (int)r.q.D, size(splits)) : 0;
+    // more splits than 256 are for the call to refuse
+    const int64_t need = splits > 1 && splits <= 256 ? (int64_t)g_scratch_bytes(size(r.NS), size(r.q.H), size(r.c.HKV), (int)r.q.D, size(splits)) : 0;
     int64_t where = 0, bytes = 0;
     if (a[17] != Py_None) {
         const at::Tensor& t = tensor(a[17], "scratch");
-        if (t.get_device() == r.q.dev) {
+        if (t.get_device() == r.q.dev && t.is_contiguous()) {
             where = address(t);
             bytes = (int64_t)t.nbytes();
         }
         if (PyObject_IsTrue(a[18]) == 1 && (where == 0 || bytes < need))
-            refuse("scratch needs " + std::to_string(need) + " bytes on device " + std::to_string(r.q.dev));
+            refuse("scratch needs " + std::to_string(need) + " contiguous bytes on device " + std::to_string(r.q.dev));
     }
     if (bytes < need) return -need;
     w.put(splits);

@@ -541,6 +541,16 @@ def test_refusals():
         ops.decode_attention_window(q, k, v, torch.empty_like(q), *good[4:])
     with pytest.raises(ValueError, match="scratch"):
         ops.decode_attention_window(*good, num_splits=4, scratch=torch.zeros(16, dtype=torch.uint8, device=DEV))
+    with pytest.raises(ValueError, match="scratch"):
+        ops.decode_attention_window(*good, num_splits=4, scratch=torch.zeros(2, 1 << 20, dtype=torch.uint8, device=DEV).t())
+    for n in (0, -1, 257, 1 << 40):
+        with pytest.raises(Exception, match="status 1"):
+            ops.decode_attention_window(*good, num_splits=n)
+    with pytest.raises(Exception, match="status 1"):
+        ops.prefill_attention_window(*good[:10], 1 << 40)
+    for i, bad in ((7, None), (8, torch.ones(1, device=DEV).half()), (3, None), (9, "one"), (10, 1.5)):
+        with pytest.raises((ValueError, TypeError)):
+            ops.prefill_attention_window(*good[:i], bad, *good[i + 1:])
     none = d["table"][:0]
     assert ops.decode_attention_window(d["q"], k, v, out, d["starts"][:1], d["seq_lens"][:0], none, *good[7:]) is out
     assert ops.prefill_attention_blk(d["q"], k, v, out, d["starts"][:1], d["seq_lens"][:0], none, *blk[7:]) is out
