@@ -339,8 +339,8 @@ prefill_visible_kernel(VisibleParams P)
                     unsigned char* x = exch + rset * kSetBytes + 16 * ln;
                     *reinterpret_cast<u32x4_t*>(x) = (u32x4_t){(uint32_t)hi[0], (uint32_t)hi[1], (uint32_t)hi[2], (uint32_t)hi[3]};
                     *reinterpret_cast<u32x4_t*>(x + 1024) = (u32x4_t){(uint32_t)hi[4], (uint32_t)hi[5], (uint32_t)hi[6], (uint32_t)hi[7]};
-                    *reinterpret_cast<u32x4_t*>(x + 2048) = (u32x4_t){(uint32_t)lo[0], (uint32_t)lo[1], (uint32_t)lo[2], (uint32_t)lo[3]};
-                    *reinterpret_cast<u32x4_t*>(x + 3072) = (u32x4_t){(uint32_t)lo[4], (uint32_t)lo[5], (uint32_t)lo[6], (uint32_t)lo[7]};
+                    *reinterpret_cast<u32x4_t*>(x + 2 * 1024) = (u32x4_t){(uint32_t)lo[0], (uint32_t)lo[1], (uint32_t)lo[2], (uint32_t)lo[3]};
+                    *reinterpret_cast<u32x4_t*>(x + 3 * 1024) = (u32x4_t){(uint32_t)lo[4], (uint32_t)lo[5], (uint32_t)lo[6], (uint32_t)lo[7]};
                     *reinterpret_cast<float*>(exch + rset * kSetBytes + 4096 + 4 * ln) = fmaxf(qk * inv, kMinFactor16);
                 }
             }
