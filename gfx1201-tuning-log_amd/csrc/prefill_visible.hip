@@ -40,6 +40,7 @@ namespace prefill_detail {
 struct VisibleParams : Params {
     const uint16_t* kv_scales;      // [blocks][block_size / 16][hkv] pairs of e8m0 bytes (K low), or null
     int window, sinks;
+    int gqa_inverse;                // 1024 / GQA, rounded up
 };
 
 // Scores of one 16-key group: K codes times the group's scale (byte KG * 2 of `scales`) against a split
@@ -199,8 +200,9 @@ prefill_visible_kernel(VisibleParams P)
 
     // head, and block within the workgroup, of row-set rset (those past the last repeat it)
     const int last_set = nbt * P.gqa - 1;
-    auto head_of = [&](int rset) { return min(rset, last_set) % P.gqa; };
-    auto block_of = [&](int rset) { return min(rset, last_set) / P.gqa; };
+    // (row-sets are below 64 and GQA at most 16, for which 1024 / GQA rounded up divides exactly)
+    auto block_of = [&](int rset) { return min(rset, last_set) * P.gqa_inverse >> 10; };
+    auto head_of = [&](int rset) { return min(rset, last_set) - block_of(rset) * P.gqa; };
     int my_block[RS];                                              // block of this wave's row-sets
 #pragma unroll
     for (int j = 0; j < RS; ++j) my_block[j] = block_of(grp * RS + j);
@@ -385,7 +387,7 @@ prefill_visible_kernel(VisibleParams P)
             for (int v = 0; v < TPW; ++v) {
                 // The next window's copies go out in TPW parts, one before each tile.
                 if (more) issue_part(i + 1, v);
-                const int tw = res * TPW + v;                    // tile within the window
+                const int tw = NR * v + res;                     // tile within the window, in the order of the copies
                 const int t = i * NT + tw;
                 const int k0 = kBN * tile_at(t);
                 if (t >= ntiles || k0 > my_hi || (k0 + kBN <= my_low && k0 >= sinks)) continue;
@@ -836,6 +838,7 @@ int prefill_visible(const void* q, int64_t q_row_stride, const void* k_cache, co
     P.kv_scales = static_cast<const uint16_t*>(kv_scales);
     P.window = window < 1 << 30 ? window : 1 << 30;     // positions less a window stay within 32 bits
     P.sinks = sinks;
+    P.gqa_inverse = (1024 + P.gqa - 1) / P.gqa;
     return launch_visible(P, KIND == kBf16, num_seqs, max_query_len, num_tokens, reinterpret_cast<hipStream_t>(stream));
 }
 
