@@ -719,10 +719,11 @@ prefill_visible_kernel(VisibleParams P)
 // A workgroup takes nb token blocks of 16, whose nb * GQA row-sets fill a shape.  More blocks share the copies of their
 // keys, start and end once, and leave fewer partial states to merge; fewer blocks split the keys over more waves, so the
 // GPU is full with fewer tokens.  The shape follows from the time that each would take, in us, fitted to 100 batches
-// (1 to 16 sequences of 100..4000, GQA 4 to 10, either cache width) at every shape; the one taken is 1.7 % slower than
-// the best on average, 39 % at most:
-//   a workgroup   9.5, and per key tile 0.2 (bf16: 0.3) for its copies and 0.65 (two row-sets a wave) or 1.2 (three)
-//                 times the filled part of its eight waves, where a wave without rows still costs three quarters;
+// (1 to 16 sequences of 100..4000, GQA 4 to 10, either cache width) at every shape; the one taken is 1.1 % slower than
+// the best on average, 32 % at most:
+//   a workgroup   9.5 (three row-sets a wave: 9.6), and per key tile 0.2 (bf16: 0.3) for its copies and 0.65 (two row-sets
+//                 a wave) or 1.2 (three) times the filled part of its eight waves, where a wave without rows still costs
+//                 three quarters;
 //   the grid      its rounds of 256 workgroups and 0.4 for the end; where the blocks cost alike (a window, pairs) half
 //                 of a last round that is not full.  Not less than the longest workgroup.
 // The host knows the queries and not the context: 192 more keys than them stand for it, and a block of a whole context
@@ -752,8 +753,9 @@ VisiblePlan plan_visible(bool b16, int gqa, int hkv, int num_seqs, int max_query
         const int block = 16 * nb, used = (nb * gqa + s.rs - 1) / s.rs;
         const double tile = (b16 ? 0.3 : 0.2) + (s.rs == 2 ? 0.65 : 1.2) * (0.75 * s.ng + 0.25 * used) / kSplitWaves;
         const double seen = (double)window + sinks + block;
-        const double most = 9.5 + tile / kBN * (limited && seen < longest ? seen : longest);
-        const double mean = limited ? most : 9.5 + tile / kBN * (0.45 * max_query_len + 192);
+        const double fixed = s.rs == 2 ? 9.5 : 9.6;
+        const double most = fixed + tile / kBN * (limited && seen < longest ? seen : longest);
+        const double mean = limited ? most : fixed + tile / kBN * (0.45 * max_query_len + 192);
         const int n = (max_query_len + block - 1) / block;
         const double blocks = num_seqs == 1 ? n : all / block + num_seqs / 2.0;
         for (int paired = 0; paired < (limited ? 1 : 2); ++paired) {
