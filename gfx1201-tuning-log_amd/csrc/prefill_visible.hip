@@ -10,8 +10,8 @@
 //
 // What bounds it: the matrix units and the softmax's exponentials; the keys of a token block are read
 // from L2 by its workgroup alone.  The shape is the key-split one of prefill_attn.hip: a workgroup of 8 waves
-// owns 16 tokens (MB: 4 / GQA blocks of them) of one kv head's query heads, or a pair of such blocks where
-// all of a causal context is seen; wave w takes row-set group w / NR, RS sets of 16 (token, head) rows,
+// owns some blocks of 16 tokens (the launch plan says how many) of one kv head's query heads, or a pair of such
+// sets where all of a causal context is seen; wave w takes row-set group w / NR, RS sets of 16 (token, head) rows,
 // and of every ring window the key tiles of residue w % NR.  Raw rows stream through an LDS ring of two windows.  Here:
 //   * a block walks the 32-key tiles that hold a visible key: those of the sinks, then those from
 //     the first query's window on.  A 16-key group inside them that holds none is not read (nor its
@@ -26,6 +26,10 @@
 //     four instructions for a row-set's eight weights).
 //   * a masked key's V must not reach a row through 0 * NaN: on masked tiles that hold a non-finite V
 //     (one test of the raw words), it is zeroed for the product and added afterwards to the rows that see it.
+// Measured in a graph: 2048 block-scaled tokens after 2048, 24 / 4 heads, 92.9 us (832 Tflop/s of visible work; a large bf16
+// product 1117), 4096 e4m3 tokens with a window of 1024 64.3, six block-scaled prompts of 37..900 46.5, five bf16
+// prompts of 100..1500 with a window of 512, 32 / 8 heads, 61.9.  The matrix units are busy 36 % of the time, the vector units
+// 52 %.  Without the exponentials the first would take 10 us less, without the second part of Q 7, without widening V 7.
 #include "fp8kv_common.h"
 #include "fp8kv_status.h"
 #include "fp8kv_diag.h"
