@@ -210,307 +210,307 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
     }
     // One segment: a split of one sequence, or what a part holds of one of its sequences.
     for (;;) {
-    int tid = threadIdx.x;
-    if constexpr (PARTS) asm volatile("" : "+v"(tid));          // nothing that follows from it is kept between segments
-    const int lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int lr = lane & 15;
-    const int lp = lane >> 4;
+        int tid = threadIdx.x;
+        if constexpr (PARTS) asm volatile("" : "+v"(tid));          // nothing that follows from it is kept between segments
+        const int lane = tid & 63;
+        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const int lr = lane & 15;
+        const int lp = lane >> 4;
 
-    int lo, hi;
-    int64_t rec0;                                      // where the split records of this (sequence, kv head) start,
-    int nrec;                                          // and how many there are
-    [[maybe_unused]] Walk walk;
-    [[maybe_unused]] int next_len = 0, next_tok = 0, groups = 0;
-    if constexpr (VISIBLE) {
-        walk = make_walk(seqlen, P.window, P.sinks);
-    }
-    if constexpr (PARTS) {
-        const int next = seq + 1 < P.ns ? seq + 1 : seq;
-        next_len = ((const_i32_t*)seq_lens)[next];
-        next_tok = ((const_i32_t*)qsl)[next];
-        groups = walk_groups(walk.nv);
-        const int w = blockIdx.x, end = part.start + part.size;
-        lo = part.start > part.base ? 16 * (part.start - part.base) : 0;
-        hi = end - part.base < groups ? 16 * (end - part.base) : walk.nv;
-        const int first = part.base >= part.start ? w : (int)((unsigned)part.base / (unsigned)part.size);
-        const int past = part.base + groups <= end ? w : (int)((unsigned)(part.base + groups - 1) / (unsigned)part.size);
-        sp = w - first;
-        nrec = past - first + 1;
-        // A record's place counts the parts and the sequences before it.
-        rec0 = (int64_t)kh * (P.parts + P.ns) + first + seq;
-    } else {
-        int tokens = seqlen;
-        if constexpr (VISIBLE) tokens = walk.nv;
-        split_span(tokens, nsplit, sp, lo, hi);
-        nrec = P.nsplit;
-        rec0 = ((int64_t)seq * P.hkv + kh) * nrec;
-    }
-    // The three steps of a chunk: its block ids, its loads, its use.
-    auto ids_of = [&](const int32_t* row, int c0, int end) {
-        if constexpr (VISIBLE) return load_chunk_ids<NG>(P, row, c0, end, walk);
-        else return load_chunk_ids<NG>(P, row, c0, end);
-    };
-    const int32_t* btrow = bt + (int64_t)seq * bt_stride;
-
-    // The wave's chunks start at c_first and step by `stride`.
-    const int stride = CH * W;
-    const int c_first = lo + CH * wave;
-    const int last = (hi - 1) & ~15;
-    // The first pair's block ids go out right behind the span (they head the dependent chain to
-    // the K/V bytes); everything below is issued while they are in flight.
-    [[maybe_unused]] ChunkIds<NG> ia, ib;
-    if constexpr (DEPTH != 1) {
-        if (c_first < hi) {
-            ia = ids_of(btrow, c_first, last);
-            ib = ids_of(btrow, c_first + stride, last);
+        int lo, hi;
+        int64_t rec0;                                      // where the split records of this (sequence, kv head) start,
+        int nrec;                                          // and how many there are
+        [[maybe_unused]] Walk walk;
+        [[maybe_unused]] int next_len = 0, next_tok = 0, groups = 0;
+        if constexpr (VISIBLE) {
+            walk = make_walk(seqlen, P.window, P.sinks);
         }
-    }
-
-    // Q^T fragments: lane (h, p) holds head h at d = 16p + (0..15) and 64 + 16p + (0..15).  Lanes
-    // h >= gqa load head 0 again: their columns of S and O are never stored, and unconditional
-    // loads leave no exec-masked write to a load's destination (which would make the compiler
-    // wait for every load in flight).  The scales are scalar loads (lgkmcnt, not vmcnt).
-    u32x4_t qf[4];
-    {
-        const __bf16* qrow = P.q + (int64_t)qtok * P.q_stride + (int64_t)(kh * gqa + (lr < gqa ? lr : 0)) * kD;
-        qf[0] = load_16(qrow + 16 * lp);
-        qf[1] = load_16(qrow + 16 * lp + 8);
-        qf[2] = load_16(qrow + 64 + 16 * lp);
-        qf[3] = load_16(qrow + 64 + 16 * lp + 8);
-    }
-    // bf16 caches carry no scales (the reference ignores k_scale and v_scale for them), block-scaled ones their own.
-    const float qk_scale = KIND != kE4m3 ? P.sm_scale * kLog2e : P.sm_scale * *(const_f32_t*)P.k_scale * kLog2e;
-    const float vs = KIND != kE4m3 ? 1.f : *(const_f32_t*)P.v_scale;
-
-    WaveState st;
-    st.m_run = neg_inf();
-    st.l_run = 0.f;
-#pragma unroll
-    for (int n = 0; n < 8; ++n) st.o[n] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-
-    if (c_first < hi) {
-        const LaneOffsets lofs = lane_offsets<B16>(P, lr, lp);
-        ChunkRegs<NG, B16> ca;
-        [[maybe_unused]] ChunkRegs<NG, B16> cb;
-        [[maybe_unused]] ChunkScales<NG> sa, sb;
-        auto issue = [&](ChunkRegs<NG, B16>& c, ChunkScales<NG>& sc, const ChunkIds<NG>& ids, int at) {
-            if constexpr (KIND == kBlk) issue_scales<NG>(sc, P, ids, kh, at, last, walk);
-            if constexpr (VISIBLE) issue_chunk<NG, KF, B16>(c, P, lofs, ids, kh, at, hi, last, walk);
-            else issue_chunk<NG, KF, B16>(c, P, lofs, ids, kh, at, hi, last);
-        };
-        auto consume = [&](const ChunkRegs<NG, B16>& c, const ChunkScales<NG>& sc, int at) {
-            if constexpr (VISIBLE) consume_visible<NG, KIND>(c, sc, st, qf, qk_scale, at, hi, walk, lp);
-            else consume_chunk<NG, B16>(c, st, qf, qk_scale, at, hi - 1, at + CH > hi, hi, lp);
-        };
-        int c0 = c_first;
-        if constexpr (DEPTH == 1) {
-            do {
-                const ChunkIds<NG> ia = ids_of(btrow, c0, last);
-                issue(ca, sa, ia, c0);
-                consume(ca, sa, c0);
-                c0 += stride;
-            } while (c0 < hi);
+        if constexpr (PARTS) {
+            const int next = seq + 1 < P.ns ? seq + 1 : seq;
+            next_len = ((const_i32_t*)seq_lens)[next];
+            next_tok = ((const_i32_t*)qsl)[next];
+            groups = walk_groups(walk.nv);
+            const int w = blockIdx.x, end = part.start + part.size;
+            lo = part.start > part.base ? 16 * (part.start - part.base) : 0;
+            hi = end - part.base < groups ? 16 * (end - part.base) : walk.nv;
+            const int first = part.base >= part.start ? w : (int)((unsigned)part.base / (unsigned)part.size);
+            const int past = part.base + groups <= end ? w : (int)((unsigned)(part.base + groups - 1) / (unsigned)part.size);
+            sp = w - first;
+            nrec = past - first + 1;
+            // A record's place counts the parts and the sequences before it.
+            rec0 = (int64_t)kh * (P.parts + P.ns) + first + seq;
         } else {
-            // Chunks in pairs: both block-id sets in one scalar round trip, both chunks' loads
-            // back to back, then chunk A is used while chunk B is still arriving.  Straight-line
-            // code up to the use of B keeps the compiler's wait counts exact.  A chunk B past hi
-            // reads one broadcast line per instruction and is not used.
-            do {
-                ids_ready(ia, ib);
-                issue(ca, sa, ia, c0);
-                issue(cb, sb, ib, c0 + stride);
-                if (c0 + 2 * stride < hi) {            // the next pair's ids, a round trip ahead
-                    ia = ids_of(btrow, c0 + 2 * stride, last);
-                    ib = ids_of(btrow, c0 + 3 * stride, last);
-                }
-                consume(ca, sa, c0);
-                if (c0 + stride >= hi) break;
-                consume(cb, sb, c0 + stride);
-                c0 += 2 * stride;
-            } while (c0 < hi);
+            int tokens = seqlen;
+            if constexpr (VISIBLE) tokens = walk.nv;
+            split_span(tokens, nsplit, sp, lo, hi);
+            nrec = P.nsplit;
+            rec0 = ((int64_t)seq * P.hkv + kh) * nrec;
         }
-    }
+        // The three steps of a chunk: its block ids, its loads, its use.
+        auto ids_of = [&](const int32_t* row, int c0, int end) {
+            if constexpr (VISIBLE) return load_chunk_ids<NG>(P, row, c0, end, walk);
+            else return load_chunk_ids<NG>(P, row, c0, end);
+        };
+        const int32_t* btrow = bt + (int64_t)seq * bt_stride;
 
-    // ---- merge the W waves in LDS ---------------------------------------------------------------
-    float l_run = st.l_run;
-    l_run = sum_xor16_32(l_run);
-    if (lp == 0 && lr < gqa) {
-        lds_ml[wave][lr][0] = st.m_run;
-        lds_ml[wave][lr][1] = l_run;
-    }
-    if (lr < gqa) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f32x4_t a = {st.o[0][i], st.o[1][i], st.o[2][i], st.o[3][i]};
-            f32x4_t b = {st.o[4][i], st.o[5][i], st.o[6][i], st.o[7][i]};
-            *reinterpret_cast<f32x4_t*>(&lds_o[wave][lr][32 * lp + 8 * i]) = a;
-            *reinterpret_cast<f32x4_t*>(&lds_o[wave][lr][32 * lp + 8 * i + 4]) = b;
+        // The wave's chunks start at c_first and step by `stride`.
+        const int stride = CH * W;
+        const int c_first = lo + CH * wave;
+        const int last = (hi - 1) & ~15;
+        // The first pair's block ids go out right behind the span (they head the dependent chain to
+        // the K/V bytes); everything below is issued while they are in flight.
+        [[maybe_unused]] ChunkIds<NG> ia, ib;
+        if constexpr (DEPTH != 1) {
+            if (c_first < hi) {
+                ia = ids_of(btrow, c_first, last);
+                ib = ids_of(btrow, c_first + stride, last);
+            }
         }
-    }
-    __syncthreads();
 
-    const int E = gqa * kD;
-    const int64_t pair = (int64_t)seq * P.hkv + kh;
-    // Each thread merges four adjacent elements of one head over the W waves' partial states: every
-    // LDS read goes out before any use (the o values of each wave in one 16-byte read, the (m, l)
-    // reads are broadcasts), and the W factors exp2(m_w - max m) serve all four elements.
-    auto merge_waves = [&](int e, f32x4_t& acc, float& mx, float& l) {
-        const int h = e / kD, d = e % kD;
-        float mw[W], lw[W];
-        f32x4_t ow[W];
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            mw[w] = lds_ml[w][h][0];
-            lw[w] = lds_ml[w][h][1];
-            ow[w] = *reinterpret_cast<const f32x4_t*>(&lds_o[w][h][d]);
+        // Q^T fragments: lane (h, p) holds head h at d = 16p + (0..15) and 64 + 16p + (0..15).  Lanes
+        // h >= gqa load head 0 again: their columns of S and O are never stored, and unconditional
+        // loads leave no exec-masked write to a load's destination (which would make the compiler
+        // wait for every load in flight).  The scales are scalar loads (lgkmcnt, not vmcnt).
+        u32x4_t qf[4];
+        {
+            const __bf16* qrow = P.q + (int64_t)qtok * P.q_stride + (int64_t)(kh * gqa + (lr < gqa ? lr : 0)) * kD;
+            qf[0] = load_16(qrow + 16 * lp);
+            qf[1] = load_16(qrow + 16 * lp + 8);
+            qf[2] = load_16(qrow + 64 + 16 * lp);
+            qf[3] = load_16(qrow + 64 + 16 * lp + 8);
         }
-        float m = neg_inf();
+        // bf16 caches carry no scales (the reference ignores k_scale and v_scale for them), block-scaled ones their own.
+        const float qk_scale = KIND != kE4m3 ? P.sm_scale * kLog2e : P.sm_scale * *(const_f32_t*)P.k_scale * kLog2e;
+        const float vs = KIND != kE4m3 ? 1.f : *(const_f32_t*)P.v_scale;
+
+        WaveState st;
+        st.m_run = neg_inf();
+        st.l_run = 0.f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) m = fmaxf(m, mw[w]);
-        const float mu = m == neg_inf() ? 0.f : m;
-        acc = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-        l = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float f = __builtin_amdgcn_exp2f(mw[w] - mu);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] += f * ow[w][i];
-            l += f * lw[w];
+        for (int n = 0; n < 8; ++n) st.o[n] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+
+        if (c_first < hi) {
+            const LaneOffsets lofs = lane_offsets<B16>(P, lr, lp);
+            ChunkRegs<NG, B16> ca;
+            [[maybe_unused]] ChunkRegs<NG, B16> cb;
+            [[maybe_unused]] ChunkScales<NG> sa, sb;
+            auto issue = [&](ChunkRegs<NG, B16>& c, ChunkScales<NG>& sc, const ChunkIds<NG>& ids, int at) {
+                if constexpr (KIND == kBlk) issue_scales<NG>(sc, P, ids, kh, at, last, walk);
+                if constexpr (VISIBLE) issue_chunk<NG, KF, B16>(c, P, lofs, ids, kh, at, hi, last, walk);
+                else issue_chunk<NG, KF, B16>(c, P, lofs, ids, kh, at, hi, last);
+            };
+            auto consume = [&](const ChunkRegs<NG, B16>& c, const ChunkScales<NG>& sc, int at) {
+                if constexpr (VISIBLE) consume_visible<NG, KIND>(c, sc, st, qf, qk_scale, at, hi, walk, lp);
+                else consume_chunk<NG, B16>(c, st, qf, qk_scale, at, hi - 1, at + CH > hi, hi, lp);
+            };
+            int c0 = c_first;
+            if constexpr (DEPTH == 1) {
+                do {
+                    const ChunkIds<NG> ia = ids_of(btrow, c0, last);
+                    issue(ca, sa, ia, c0);
+                    consume(ca, sa, c0);
+                    c0 += stride;
+                } while (c0 < hi);
+            } else {
+                // Chunks in pairs: both block-id sets in one scalar round trip, both chunks' loads
+                // back to back, then chunk A is used while chunk B is still arriving.  Straight-line
+                // code up to the use of B keeps the compiler's wait counts exact.  A chunk B past hi
+                // reads one broadcast line per instruction and is not used.
+                do {
+                    ids_ready(ia, ib);
+                    issue(ca, sa, ia, c0);
+                    issue(cb, sb, ib, c0 + stride);
+                    if (c0 + 2 * stride < hi) {            // the next pair's ids, a round trip ahead
+                        ia = ids_of(btrow, c0 + 2 * stride, last);
+                        ib = ids_of(btrow, c0 + 3 * stride, last);
+                    }
+                    consume(ca, sa, c0);
+                    if (c0 + stride >= hi) break;
+                    consume(cb, sb, c0 + stride);
+                    c0 += 2 * stride;
+                } while (c0 < hi);
+            }
         }
-        mx = m;
-    };
-    auto finish = [&] {
-    if (nrec == 1) {
-        for (int e0 = 0; e0 < E; e0 += 4 * T) {
-            const int e = e0 + 4 * tid;
-            if (e >= E) break;
-            f32x4_t acc;
-            float m, l;
-            merge_waves(e, acc, m, l);
+
+        // ---- merge the W waves in LDS ---------------------------------------------------------------
+        float l_run = st.l_run;
+        l_run = sum_xor16_32(l_run);
+        if (lp == 0 && lr < gqa) {
+            lds_ml[wave][lr][0] = st.m_run;
+            lds_ml[wave][lr][1] = l_run;
+        }
+        if (lr < gqa) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float r = l > 0.f ? acc[i] * vs / l : 0.f;
-                P.out[(int64_t)qtok * P.o_stride + (int64_t)(kh * gqa) * kD + e + i] = (__bf16)r;
+                f32x4_t a = {st.o[0][i], st.o[1][i], st.o[2][i], st.o[3][i]};
+                f32x4_t b = {st.o[4][i], st.o[5][i], st.o[6][i], st.o[7][i]};
+                *reinterpret_cast<f32x4_t*>(&lds_o[wave][lr][32 * lp + 8 * i]) = a;
+                *reinterpret_cast<f32x4_t*>(&lds_o[wave][lr][32 * lp + 8 * i + 4]) = b;
             }
         }
-        return;
-    }
+        __syncthreads();
 
-    // ---- this split's partial record -------------------------------------------------------------
-    const int rf = record_floats(gqa);
-    float* rec = P.part + (rec0 + sp) * rf;
-    for (int e0 = 0; e0 < E; e0 += 4 * T) {
-        const int e = e0 + 4 * tid;
-        if (e >= E) break;
-        f32x4_t acc;
-        float m, l;
-        merge_waves(e, acc, m, l);
-        store_coherent4(rec + e, acc);
-        if (e % kD == 0) store_coherent2(rec + E + 2 * (e / kD), m, l);
-    }
-
-    // ---- ticket: the last split of this (sequence, kv head) merges --------------------------------
-    // The records were written with device-coherent stores; once they have completed
-    // (vmcnt(0)) the ticket increment may be observed.  The merging workgroup reads them with
-    // device-coherent loads issued after it has seen the final ticket value.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (tid == 0) {
-        const uint32_t t = __hip_atomic_fetch_add(P.counters + ticket_slot(pair), 1u, __ATOMIC_RELAXED,
-                                                  __HIP_MEMORY_SCOPE_AGENT);
-        lds_last = (t == (uint32_t)(nrec - 1)) ? 1 : 0;
-    }
-    __syncthreads();
-    if (!lds_last) return;
-
-    const float* recs_all = P.part + rec0 * rf;
-    const int64_t out_row = (int64_t)qtok * P.o_stride + (int64_t)(kh * gqa) * kD;
-    if (nrec <= 32) {
-        if (nrec <= 2)
-            merge_regs<2, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
-        else if (nrec <= 4)
-            merge_regs<4, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
-        else if (nrec <= 8)
-            merge_regs<8, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
-        else if (nrec <= 16)
-            merge_regs<16, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
-        else
-            merge_regs<32, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
-        if (tid == 0)
-            __hip_atomic_store(P.counters + ticket_slot(pair), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        return;
-    }
-
-    // More than 32 splits (only when the caller asks for them): one round trip per kMergeBatch
-    // splits: m and l of every split go to LDS once
-    // (one load per split and head), each thread loads the o values of its own elements
-    // tid + T j, and both are in flight together before the barrier.
-    const float* recs = P.part + rec0 * rf;
-    const int NSG = nrec * gqa;
-    float* wm = &lds_o[0][0][0];            // [nsplit][gqa] m, then [nsplit][gqa] l
-    float m[EPT], acc[EPT], l[EPT];
+        const int E = gqa * kD;
+        const int64_t pair = (int64_t)seq * P.hkv + kh;
+        // Each thread merges four adjacent elements of one head over the W waves' partial states: every
+        // LDS read goes out before any use (the o values of each wave in one 16-byte read, the (m, l)
+        // reads are broadcasts), and the W factors exp2(m_w - max m) serve all four elements.
+        auto merge_waves = [&](int e, f32x4_t& acc, float& mx, float& l) {
+            const int h = e / kD, d = e % kD;
+            float mw[W], lw[W];
+            f32x4_t ow[W];
 #pragma unroll
-    for (int j = 0; j < EPT; ++j) { m[j] = neg_inf(); acc[j] = 0.f; l[j] = 0.f; }
-    for (int s0 = 0; s0 < nrec; s0 += kMergeBatch) {
-        float ov[EPT][kMergeBatch];
-#pragma unroll
-        for (int j = 0; j < EPT; ++j) {
-            const int e = tid + T * j;
-#pragma unroll
-            for (int b = 0; b < kMergeBatch; ++b) {
-                const int s2 = s0 + b < nrec ? s0 + b : nrec - 1;
-                ov[j][b] = e < E ? load_coherent(recs + (int64_t)s2 * rf + e) : 0.f;
+            for (int w = 0; w < W; ++w) {
+                mw[w] = lds_ml[w][h][0];
+                lw[w] = lds_ml[w][h][1];
+                ow[w] = *reinterpret_cast<const f32x4_t*>(&lds_o[w][h][d]);
             }
-        }
-        if (s0 == 0) {
-            for (int i = tid; i < NSG; i += T) {
-                const int s2 = i / gqa, h = i % gqa;
-                wm[i] = load_coherent(recs + (int64_t)s2 * rf + E + 2 * h);
-                wm[NSG + i] = load_coherent(recs + (int64_t)s2 * rf + E + 2 * h + 1);
+            float m = neg_inf();
+#pragma unroll
+            for (int w = 0; w < W; ++w) m = fmaxf(m, mw[w]);
+            const float mu = m == neg_inf() ? 0.f : m;
+            acc = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+            l = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float f = __builtin_amdgcn_exp2f(mw[w] - mu);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] += f * ow[w][i];
+                l += f * lw[w];
+            }
+            mx = m;
+        };
+        auto finish = [&] {
+            if (nrec == 1) {
+                for (int e0 = 0; e0 < E; e0 += 4 * T) {
+                    const int e = e0 + 4 * tid;
+                    if (e >= E) break;
+                    f32x4_t acc;
+                    float m, l;
+                    merge_waves(e, acc, m, l);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float r = l > 0.f ? acc[i] * vs / l : 0.f;
+                        P.out[(int64_t)qtok * P.o_stride + (int64_t)(kh * gqa) * kD + e + i] = (__bf16)r;
+                    }
+                }
+                return;
+            }
+
+            // ---- this split's partial record -------------------------------------------------------------
+            const int rf = record_floats(gqa);
+            float* rec = P.part + (rec0 + sp) * rf;
+            for (int e0 = 0; e0 < E; e0 += 4 * T) {
+                const int e = e0 + 4 * tid;
+                if (e >= E) break;
+                f32x4_t acc;
+                float m, l;
+                merge_waves(e, acc, m, l);
+                store_coherent4(rec + e, acc);
+                if (e % kD == 0) store_coherent2(rec + E + 2 * (e / kD), m, l);
+            }
+
+            // ---- ticket: the last split of this (sequence, kv head) merges --------------------------------
+            // The records were written with device-coherent stores; once they have completed
+            // (vmcnt(0)) the ticket increment may be observed.  The merging workgroup reads them with
+            // device-coherent loads issued after it has seen the final ticket value.
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (tid == 0) {
+                const uint32_t t = __hip_atomic_fetch_add(P.counters + ticket_slot(pair), 1u, __ATOMIC_RELAXED,
+                                                          __HIP_MEMORY_SCOPE_AGENT);
+                lds_last = (t == (uint32_t)(nrec - 1)) ? 1 : 0;
             }
             __syncthreads();
-        }
-#pragma unroll
-        for (int j = 0; j < EPT; ++j) {
-            const int h = (tid + T * j) / kD;
-            if (h >= gqa) continue;
-#pragma unroll
-            for (int b = 0; b < kMergeBatch; ++b) {
-                if (s0 + b >= nrec) break;
-                const float ms = wm[(s0 + b) * gqa + h];
-                const float mn = fmaxf(m[j], ms);
-                const float mu = mn == neg_inf() ? 0.f : mn;
-                const float a = __builtin_amdgcn_exp2f(m[j] - mu);
-                const float f = __builtin_amdgcn_exp2f(ms - mu);
-                acc[j] = acc[j] * a + f * ov[j][b];
-                l[j] = l[j] * a + f * wm[NSG + (s0 + b) * gqa + h];
-                m[j] = mn;
+            if (!lds_last) return;
+
+            const float* recs_all = P.part + rec0 * rf;
+            const int64_t out_row = (int64_t)qtok * P.o_stride + (int64_t)(kh * gqa) * kD;
+            if (nrec <= 32) {
+                if (nrec <= 2)
+                    merge_regs<2, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+                else if (nrec <= 4)
+                    merge_regs<4, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+                else if (nrec <= 8)
+                    merge_regs<8, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+                else if (nrec <= 16)
+                    merge_regs<16, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+                else
+                    merge_regs<32, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+                if (tid == 0)
+                    __hip_atomic_store(P.counters + ticket_slot(pair), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                return;
             }
-        }
-    }
+
+            // More than 32 splits (only when the caller asks for them): one round trip per kMergeBatch
+            // splits: m and l of every split go to LDS once
+            // (one load per split and head), each thread loads the o values of its own elements
+            // tid + T j, and both are in flight together before the barrier.
+            const float* recs = P.part + rec0 * rf;
+            const int NSG = nrec * gqa;
+            float* wm = &lds_o[0][0][0];            // [nsplit][gqa] m, then [nsplit][gqa] l
+            float m[EPT], acc[EPT], l[EPT];
 #pragma unroll
-    for (int j = 0; j < EPT; ++j) {
-        const int e = tid + T * j;
-        if (e < E) {
-            const float r = l[j] > 0.f ? acc[j] * vs / l[j] : 0.f;
-            P.out[(int64_t)qtok * P.o_stride + (int64_t)(kh * gqa) * kD + e] = (__bf16)r;
+            for (int j = 0; j < EPT; ++j) { m[j] = neg_inf(); acc[j] = 0.f; l[j] = 0.f; }
+            for (int s0 = 0; s0 < nrec; s0 += kMergeBatch) {
+                float ov[EPT][kMergeBatch];
+#pragma unroll
+                for (int j = 0; j < EPT; ++j) {
+                    const int e = tid + T * j;
+#pragma unroll
+                    for (int b = 0; b < kMergeBatch; ++b) {
+                        const int s2 = s0 + b < nrec ? s0 + b : nrec - 1;
+                        ov[j][b] = e < E ? load_coherent(recs + (int64_t)s2 * rf + e) : 0.f;
+                    }
+                }
+                if (s0 == 0) {
+                    for (int i = tid; i < NSG; i += T) {
+                        const int s2 = i / gqa, h = i % gqa;
+                        wm[i] = load_coherent(recs + (int64_t)s2 * rf + E + 2 * h);
+                        wm[NSG + i] = load_coherent(recs + (int64_t)s2 * rf + E + 2 * h + 1);
+                    }
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int j = 0; j < EPT; ++j) {
+                    const int h = (tid + T * j) / kD;
+                    if (h >= gqa) continue;
+#pragma unroll
+                    for (int b = 0; b < kMergeBatch; ++b) {
+                        if (s0 + b >= nrec) break;
+                        const float ms = wm[(s0 + b) * gqa + h];
+                        const float mn = fmaxf(m[j], ms);
+                        const float mu = mn == neg_inf() ? 0.f : mn;
+                        const float a = __builtin_amdgcn_exp2f(m[j] - mu);
+                        const float f = __builtin_amdgcn_exp2f(ms - mu);
+                        acc[j] = acc[j] * a + f * ov[j][b];
+                        l[j] = l[j] * a + f * wm[NSG + (s0 + b) * gqa + h];
+                        m[j] = mn;
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < EPT; ++j) {
+                const int e = tid + T * j;
+                if (e < E) {
+                    const float r = l[j] > 0.f ? acc[j] * vs / l[j] : 0.f;
+                    P.out[(int64_t)qtok * P.o_stride + (int64_t)(kh * gqa) * kD + e] = (__bf16)r;
+                }
+            }
+            if (tid == 0)
+                __hip_atomic_store(P.counters + ticket_slot(pair), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        };
+        finish();
+        if constexpr (PARTS) {
+            part.base += groups;
+            ++seq;
+            if (part.base >= part.start + part.size || seq >= P.ns) return;
+            seqlen = next_len;
+            qtok = next_tok;
+            __syncthreads();                               // the next segment's states go where this one's were read
+        } else {
+            return;
         }
-    }
-    if (tid == 0)
-        __hip_atomic_store(P.counters + ticket_slot(pair), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    };
-    finish();
-    if constexpr (PARTS) {
-        part.base += groups;
-        ++seq;
-        if (part.base >= part.start + part.size || seq >= P.ns) return;
-        seqlen = next_len;
-        qtok = next_tok;
-        __syncthreads();                               // the next segment's states go where this one's were read
-    } else {
-        return;
-    }
     }
 }
 
