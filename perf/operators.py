@@ -195,18 +195,12 @@ def _starts(lengths):
     return got
 
 
-_framework = None
-
-
 def _ops():
-    global _framework
-    if _framework is None:                    # a program imports the framework once
-        path = os.path.join(os.getcwd(), "gfx1201-tuning-log_amd")
-        if path not in sys.path:
-            sys.path.insert(0, path)
-        from fp8kv_amd import ops
-        _framework = ops
-    return _framework
+    path = os.path.join(os.getcwd(), "gfx1201-tuning-log_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from fp8kv_amd import ops
+    return ops
 
 
 def prepare(case, seed):
