@@ -247,6 +247,9 @@ struct Attention {
 Attention attention_lead(Words& w, PyObject* const* a, bool blk)
 {
     const at::Tensor &q = tensor(a[3], "q"), &out = tensor(a[6], "out");
+    // the calls write the rows of q in out; looked at first, which needs no device
+    if (q.dim() > 0 && out.dim() > 0 && out.size(0) < q.size(0))
+        refuse("out has " + std::to_string(out.size(0)) + " rows, fewer than q's " + std::to_string(q.size(0)));
     Attention r{rows(q, "q"), {}, 0};
     const Rows o = rows(out, "out");
     if (!(o.H == r.q.H && o.D == r.q.D && o.dev == r.q.dev)) refuse("out must be [T, HQ, D] of q's heads and device");

@@ -495,6 +495,7 @@ def decode_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
                             scratch: torch.Tensor | None = None) -> torch.Tensor:
     """``decode_attention`` where the query of sequence s, at position p = seq_lens[s] - 1, sees only the keys
     t > p - window and the first ``sinks`` ones (window 0: all).  Caches e4m3 with per-tensor scales, or bf16.
+    ``out`` has a row for every row of ``q`` (here and in the three calls below).
 
     Only the visible keys are read; block-table entries of blocks that hold none may be anything.  A window bounds
     the work, so ``max_seq_len`` is needed only without one (and then read from ``seq_lens``, which synchronises)."""
