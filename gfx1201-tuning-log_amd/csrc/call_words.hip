@@ -80,3 +80,12 @@ extern "C" int fp8kv_call(int entry, const int64_t* words, int count)
     if (entry < 0 || entry >= kNumEntries || !words || count != kEntries[entry].count) return FP8KV_ERR_ARG;
     return kEntries[entry].call(words);
 }
+
+extern "C" unsigned long long fp8kv_stream_capture(void* stream)
+{
+    if (!stream) return 0;                          // the null stream cannot be captured
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(reinterpret_cast<hipStream_t>(stream), &status, &id) != hipSuccess) return 0;
+    return status == hipStreamCaptureStatusNone ? 0 : id + 1;
+}

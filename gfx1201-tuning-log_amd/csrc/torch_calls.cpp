@@ -15,6 +15,7 @@ namespace {
 int (*g_call)(int, const int64_t*, int) = nullptr;
 int (*g_splits)(int, int, int, int, int, int) = nullptr;
 size_t (*g_scratch_bytes)(int, int, int, int, int) = nullptr;
+unsigned long long (*g_capture)(void*) = nullptr;
 
 struct Refused {
     std::string what;
@@ -277,8 +278,9 @@ Attention attention_lead(Words& w, PyObject* const* a, bool blk)
     return r;
 }
 
-// [attention_lead], num_splits or None, max_seq_len (0: not known), scratch or None, whether the scratch is the caller's.
-// A positive result is a status; a negative one the bytes of scratch that the call needs, and has not been given.
+// [attention_lead], num_splits or None, max_seq_len (0: not known), scratch or None, whether it is for this call.
+// A positive result is a status; a negative one the bytes of scratch that the call needs, and has not been given: under
+// capture, the buffer that the stream's eager calls use (the last argument false) is not taken.
 int64_t decode(PyObject* const* a, bool blk)
 {
     Words w;
@@ -291,13 +293,15 @@ int64_t decode(PyObject* const* a, bool blk)
     // more splits than 256 are for the call to refuse
     const int64_t need = splits > 1 && splits <= 256 ? (int64_t)g_scratch_bytes(size(r.NS), size(r.q.H), size(r.c.HKV), (int)r.q.D, size(splits)) : 0;
     int64_t where = 0, bytes = 0;
+    const bool given = PyObject_IsTrue(a[18]) == 1;
+    if (need > 0 && !given && g_capture(reinterpret_cast<void*>(integer(a[2])))) return -need;
     if (a[17] != Py_None) {
         const at::Tensor& t = tensor(a[17], "scratch");
         if (t.get_device() == r.q.dev && t.is_contiguous()) {
             where = address(t);
             bytes = (int64_t)t.nbytes();
         }
-        if (PyObject_IsTrue(a[18]) == 1 && (where == 0 || bytes < need))
+        if (given && (where == 0 || bytes < need))
             refuse("scratch needs " + std::to_string(need) + " contiguous bytes on device " + std::to_string(r.q.dev));
     }
     if (bytes < need) return -need;
@@ -348,13 +352,14 @@ PyObject* py_decode_blk(PyObject*, PyObject* const* a, Py_ssize_t n) { return gu
 PyObject* py_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 16, [&] { return prefill(a, false); }); }
 PyObject* py_prefill_blk(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded(n, 16, [&] { return prefill(a, true); }); }
 
-// Addresses of fp8kv_call, fp8kv_decode_visible_splits and fp8kv_decode_scratch_bytes.
+// Addresses of fp8kv_call, fp8kv_decode_visible_splits, fp8kv_decode_scratch_bytes and fp8kv_stream_capture.
 PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n)
 {
-    return guarded(n, 3, [&] {
+    return guarded(n, 4, [&] {
         g_call = reinterpret_cast<decltype(g_call)>(integer(a[0]));
         g_splits = reinterpret_cast<decltype(g_splits)>(integer(a[1]));
         g_scratch_bytes = reinterpret_cast<decltype(g_scratch_bytes)>(integer(a[2]));
+        g_capture = reinterpret_cast<decltype(g_capture)>(integer(a[3]));
         return 0;
     });
 }

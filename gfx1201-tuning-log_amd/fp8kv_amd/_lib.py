@@ -82,6 +82,7 @@ SIGNATURES: dict[str, tuple] = {
     # these calls with their arguments packed into 64-bit words (csrc/call_words.hip)
     "fp8kv_call_entry": (_c_i, [ctypes.c_char_p]),
     "fp8kv_call": (_c_i, [_c_i, ctypes.c_char_p, _c_i]),
+    "fp8kv_stream_capture": (ctypes.c_ulonglong, [_c_vp]),
     # layer epilogues (csrc/epilogues.hip, h4mv_silu_mul in csrc/h4mv.hip)
     "fp8kv_fused_add_rmsnorm": (_c_i, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_i, _c_i,
                                        _c_f, _c_i, _c_vp]),
@@ -199,7 +200,8 @@ def load_calls():
             module = importlib.util.module_from_spec(spec)
             loader.exec_module(module)
             module.bind(*(ctypes.cast(fn, ctypes.c_void_p).value for fn in
-                          (lib.fp8kv_call, lib.fp8kv_decode_visible_splits, lib.fp8kv_decode_scratch_bytes)))
+                          (lib.fp8kv_call, lib.fp8kv_decode_visible_splits, lib.fp8kv_decode_scratch_bytes,
+                           lib.fp8kv_stream_capture)))
             _calls = module
         return _calls
 

@@ -396,15 +396,19 @@ def _native(method: str, *names: str) -> tuple:
     return getattr(_lib.load_calls(), method), *(lib.fp8kv_call_entry(n.encode()) for n in names)
 
 
-def _run(native: tuple, dev: int, *args) -> int:
-    """The native call on the current stream of device ``dev``, whichever device is current."""
-    if dev < 0:                                   # a CPU tensor, which the call refuses
-        return native[0](*native[1:], 0, *args)
-    if dev == _current_device():
-        return native[0](*native[1:], _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream,
-                         *args)
+def _stream_of(dev: int) -> int:
+    """The current stream of device ``dev`` (0 for a CPU tensor's -1)."""
+    if dev < 0:
+        return 0
+    return _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream
+
+
+def _run(native: tuple, dev: int, stream: int, *args) -> int:
+    """The native call on ``stream`` of device ``dev``, whichever device is current; the call refuses CPU tensors."""
+    if dev < 0 or dev == _current_device():
+        return native[0](*native[1:], stream, *args)
     with torch.cuda.device(dev):
-        return native[0](*native[1:], torch.cuda.current_stream(dev).cuda_stream, *args)
+        return native[0](*native[1:], stream, *args)
 
 
 def _scale_pair(k_scale, v_scale, cache: torch.Tensor) -> tuple:
@@ -429,7 +433,8 @@ def rope_append(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tensor, 
     if q is not None and q_out is None:
         q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
     k_scale, v_scale = _scale_pair(k_scale, v_scale, k_cache)
-    st = _run(_native("rope_append", "fp8kv_rope_append", "fp8kv_rope_append_bf16"), key.get_device(), q, key, value, k_cache,
+    dev = key.get_device()
+    st = _run(_native("rope_append", "fp8kv_rope_append", "fp8kv_rope_append_bf16"), dev, _stream_of(dev), q, key, value, k_cache,
               v_cache, positions, cos_sin, q_out, interleaved, slot_mapping, k_scale, v_scale)
     if st:
         _lib.check("fp8kv_rope_append", st)
@@ -451,7 +456,8 @@ def rope_append_blk(q: torch.Tensor | None, key: torch.Tensor, value: torch.Tens
     Rows of q_out behind the last sequence are left as they were (fp8kv_rope_append_blk)."""
     if q is not None and q_out is None:
         q_out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    st = _run(_native("rope_append_blk", "fp8kv_rope_append_blk"), key.get_device(), q, key, value, k_cache, v_cache, positions,
+    dev = key.get_device()
+    st = _run(_native("rope_append_blk", "fp8kv_rope_append_blk"), dev, _stream_of(dev), q, key, value, k_cache, v_cache, positions,
               cos_sin, q_out, interleaved, kv_scales, query_start_loc, seq_lens, block_table)
     if st:
         _lib.check("fp8kv_rope_append_blk", st)
@@ -472,6 +478,31 @@ def _longest_query(starts: torch.Tensor) -> int:
     return int((starts[1:] - starts[:-1]).max().item()) if starts.numel() > 1 else 0
 
 
+# Scratch of the decode calls below, by (device, stream): calls of one stream follow one another, those of two streams
+# may run at once.  A captured call runs when and where its graph is replayed, so its scratch is the capture's own.
+_stream_scratch: dict = {}          # (device, stream) -> buffer of eager calls
+_capture_scratch: dict = {}         # (device, stream) -> (number of the latest capture, its buffer)
+
+
+def _scratch_for(nbytes: int, device: torch.device, stream: int, capture: int) -> torch.Tensor:
+    """Scratch of at least ``nbytes`` for a call on ``stream``, the current one, which records into capture number
+    ``capture`` (0: none).  Under capture its memory is the graph's, and its tickets are zeroed whenever that is replayed;
+    a buffer of the capture before is let go, which leaves it to that graph's pool."""
+    key = (device.index, stream)
+    if capture:
+        number, buf = _capture_scratch.get(key, (0, None))
+        if number != capture or buf.numel() < nbytes:
+            buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            decode_scratch_reset(buf[:_DECODE_TICKET_BYTES])
+            _capture_scratch[key] = (capture, buf)
+        return buf
+    buf = _stream_scratch.get(key)
+    if buf is None or buf.numel() < nbytes:
+        size = max(nbytes, DECODE_SCRATCH_MIN_BYTES, 0 if buf is None else 2 * buf.numel())
+        buf = _stream_scratch[key] = torch.zeros(size, dtype=torch.uint8, device=device)
+    return buf
+
+
 def _decode(native, name, q, k_cache, v_cache, out, starts, seq_lens, block_table, scales, sm_scale, window, sinks, num_splits,
             max_seq_len, scratch):
     if max_seq_len is None:
@@ -480,10 +511,13 @@ def _decode(native, name, q, k_cache, v_cache, out, starts, seq_lens, block_tabl
         else:
             max_seq_len = 0
     dev = q.get_device()
+    stream = _stream_of(dev)
     args = (q, k_cache, v_cache, out, starts, seq_lens, block_table, *scales, sm_scale, window, sinks, num_splits, max_seq_len)
-    st = _run(native, dev, *args, _scratch_cache.get(("cuda", dev)) if scratch is None else scratch, scratch is not None)
+    st = _run(native, dev, stream, *args, _stream_scratch.get((dev, stream)) if scratch is None else scratch, scratch is not None)
     if st < 0:                                    # the bytes of scratch it needs
-        st = _run(native, dev, *args, _call_scratch(-st, q.device), True)
+        with torch.cuda.device(dev):
+            buf = _scratch_for(-st, q.device, stream, _lib.load().fp8kv_stream_capture(stream))
+        st = _run(native, dev, stream, *args, buf, True)
     if st:
         _lib.check(name, st)
 
@@ -498,7 +532,9 @@ def decode_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     ``out`` has a row for every row of ``q`` (here and in the three calls below).
 
     Only the visible keys are read; block-table entries of blocks that hold none may be anything.  A window bounds
-    the work, so ``max_seq_len`` is needed only without one (and then read from ``seq_lens``, which synchronises)."""
+    the work, so ``max_seq_len`` is needed only without one (and then read from ``seq_lens``, which synchronises).
+    ``scratch`` defaults to a buffer of the current stream's, or of the graph's under capture, so that calls on two
+    streams and replays may run at once; one that is given is for one call at a time."""
     _decode(_native("decode", "fp8kv_decode_attn_window", "fp8kv_decode_attn_window_bf16"), "fp8kv_decode_attn_window", q, k_cache,
             v_cache, out, query_start_loc, seq_lens, block_table, _scale_pair(k_scale, v_scale, k_cache), sm_scale, window, sinks,
             num_splits, max_seq_len, scratch)
@@ -512,8 +548,9 @@ def prefill_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: to
     """``prefill_attention_varlen`` where the query at position p sees the keys t <= p with t > p - window
     or t < sinks (window 0: all t <= p).  Caches e4m3 with per-tensor scales, or bf16."""
     k_scale, v_scale = _scale_pair(k_scale, v_scale, k_cache)
-    st = _run(_native("prefill", "fp8kv_prefill_attn_window", "fp8kv_prefill_attn_window_bf16"), q.get_device(), q, k_cache, v_cache,
-              out, cu_seqlens_q, seq_lens, block_table, k_scale, v_scale, sm_scale, window, sinks,
+    dev = q.get_device()
+    st = _run(_native("prefill", "fp8kv_prefill_attn_window", "fp8kv_prefill_attn_window_bf16"), dev, _stream_of(dev), q, k_cache,
+              v_cache, out, cu_seqlens_q, seq_lens, block_table, k_scale, v_scale, sm_scale, window, sinks,
               _longest_query(cu_seqlens_q) if max_query_len is None else max_query_len)
     if st:
         _lib.check("fp8kv_prefill_attn_window", st)
@@ -538,8 +575,9 @@ def prefill_attention_blk(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
                           max_query_len: int | None = None) -> torch.Tensor:
     """``prefill_attention_varlen`` over the block-scaled e4m3 cache that ``rope_append_blk`` writes, with ``window``
     and ``sinks`` as in ``prefill_attention_window``."""
-    st = _run(_native("prefill_blk", "fp8kv_prefill_attn_blk", "fp8kv_prefill_attn_blk"), q.get_device(), q, k_cache, v_cache, out,
-              cu_seqlens_q, seq_lens, block_table, kv_scales, None, sm_scale, window, sinks,
+    dev = q.get_device()
+    st = _run(_native("prefill_blk", "fp8kv_prefill_attn_blk", "fp8kv_prefill_attn_blk"), dev, _stream_of(dev), q, k_cache, v_cache,
+              out, cu_seqlens_q, seq_lens, block_table, kv_scales, None, sm_scale, window, sinks,
               _longest_query(cu_seqlens_q) if max_query_len is None else max_query_len)
     if st:
         _lib.check("fp8kv_prefill_attn_blk", st)

@@ -627,6 +627,10 @@ int fp8kv_rerank_exact(const void* E, int64_t e_row_stride, int V, const void* X
 int fp8kv_call_entry(const char* name);
 int fp8kv_call(int entry, const int64_t* words, int count);
 
+/* A number of the capture that `stream` records into, another one for every capture; 0 where it records none.  For
+ * bindings that give every captured graph a scratch of its own. */
+unsigned long long fp8kv_stream_capture(void* stream);
+
 #ifdef __cplusplus
 }
 #endif
