@@ -108,13 +108,22 @@ __host__ __device__ inline void split_span(int seqlen, int nsplit, int sp, int& 
     hi = seqlen < lo + span ? seqlen : lo + span;
 }
 
+// The output element of a sum `a` of weighted values and its sum of weights `l`.  A row that sees no key has l = 0 and is
+// zero.  A NaN score makes l NaN, which reaches the output of the visible-key calls (NAN_ROWS); the calls over whole
+// contexts have always written zeros there.
+template <bool NAN_ROWS>
+__device__ __forceinline__ float normalised(float a, float vs, float l)
+{
+    return (NAN_ROWS ? l != 0.f : l > 0.f) ? a * vs / l : 0.f;
+}
+
 // Final merge of up to SMAX split records in one round trip, with no LDS and no barrier.  Thread t
 // takes the two adjacent elements 2t, 2t + 1 (+ 2T per pass), so the 128 elements of a wave are one
 // head.  Each split's two o values (one 8-byte load) and, in lane s, split s's (m, l) pair of the
 // wave's head are requested together with straight-line loads (split indices past nsplit repeat
 // the last split); the wave reads the pairs with readlane, computes the factors exp2(m_s - max m)
 // once for both elements, and adds every split's term independently of the others.
-template <int SMAX, int T>
+template <int SMAX, int T, bool NAN_ROWS>
 __device__ __forceinline__ void merge_regs(const Params& P, const float* recs, int ns, int rf, int E, int tid, float vs,
                                             int64_t out_row)
 {
@@ -151,10 +160,8 @@ __device__ __forceinline__ void merge_regs(const Params& P, const float* recs, i
                 l += f * ls[s];
             }
         }
-        const float r0 = l > 0.f ? a0 * vs / l : 0.f;
-        const float r1 = l > 0.f ? a1 * vs / l : 0.f;
-        P.out[out_row + e] = (__bf16)r0;
-        P.out[out_row + e + 1] = (__bf16)r1;
+        P.out[out_row + e] = (__bf16)normalised<NAN_ROWS>(a0, vs, l);
+        P.out[out_row + e + 1] = (__bf16)normalised<NAN_ROWS>(a1, vs, l);
     }
 }
 
@@ -390,7 +397,7 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
                     merge_waves(e, acc, m, l);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float r = l > 0.f ? acc[i] * vs / l : 0.f;
+                        const float r = normalised<VISIBLE>(acc[i], vs, l);
                         P.out[(int64_t)qtok * P.o_stride + (int64_t)(kh * gqa) * kD + e + i] = (__bf16)r;
                     }
                 }
@@ -428,15 +435,15 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
             const int64_t out_row = (int64_t)qtok * P.o_stride + (int64_t)(kh * gqa) * kD;
             if (nrec <= 32) {
                 if (nrec <= 2)
-                    merge_regs<2, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+                    merge_regs<2, T, VISIBLE>(P, recs_all, nrec, rf, E, tid, vs, out_row);
                 else if (nrec <= 4)
-                    merge_regs<4, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+                    merge_regs<4, T, VISIBLE>(P, recs_all, nrec, rf, E, tid, vs, out_row);
                 else if (nrec <= 8)
-                    merge_regs<8, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+                    merge_regs<8, T, VISIBLE>(P, recs_all, nrec, rf, E, tid, vs, out_row);
                 else if (nrec <= 16)
-                    merge_regs<16, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+                    merge_regs<16, T, VISIBLE>(P, recs_all, nrec, rf, E, tid, vs, out_row);
                 else
-                    merge_regs<32, T>(P, recs_all, nrec, rf, E, tid, vs, out_row);
+                    merge_regs<32, T, VISIBLE>(P, recs_all, nrec, rf, E, tid, vs, out_row);
                 if (tid == 0)
                     __hip_atomic_store(P.counters + ticket_slot(pair), 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 return;
@@ -493,7 +500,7 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
             for (int j = 0; j < EPT; ++j) {
                 const int e = tid + T * j;
                 if (e < E) {
-                    const float r = l[j] > 0.f ? acc[j] * vs / l[j] : 0.f;
+                    const float r = normalised<VISIBLE>(acc[j], vs, l[j]);
                     P.out[(int64_t)qtok * P.o_stride + (int64_t)(kh * gqa) * kD + e] = (__bf16)r;
                 }
             }
