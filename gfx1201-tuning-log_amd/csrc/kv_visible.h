@@ -11,8 +11,11 @@
 // two per 16 tokens, kv head and tensor as an e8m0 byte).  K's scale joins the factor that its group's
 // scores are multiplied by anyway; V's goes into its widening to bf16, which stays exact.
 //
-// The probabilities enter P.V as bf16 hi + lo parts (error 2^-17 of each instead of 2^-9): one token's
-// worth of queries leaves the matrix units idle most of the time, so the second MFMA costs nothing.
+// The probabilities enter P.V as bf16 hi + lo parts (error at most 2^-16 of each; of one rounded bf16 2^-8): one token's
+// worth of queries leaves the matrix units idle most of the time, so the second MFMA costs nothing.  hi is cut off,
+// not rounded, and the last bit of the fp32 weight is set (2^-23 of it), so that lo has the weight's sign and is
+// not 0: an infinite V is then infinite in both products.  (Rounded to nearest, lo is 0 or negative for half of the
+// weights, and 0 * inf or inf - inf is NaN.)  Where a weight is next to nothing (below 2^-100) the product may be NaN.
 #pragma once
 #include "kv_chunk.h"
 
@@ -197,10 +200,11 @@ __device__ __forceinline__ void consume_visible(const ChunkRegs<NG, KIND == kBf1
         u32x4_t hi4, lo4;
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-            const float a = s[2 * G + (d >> 1)][2 * (d & 1)], b = s[2 * G + (d >> 1)][2 * (d & 1) + 1];
-            const uint32_t h = pack_bf16x2(a, b);
-            hi4[d] = h;
-            lo4[d] = pack_bf16x2(a - __uint_as_float(h << 16), b - __uint_as_float(h & 0xFFFF0000u));
+            const uint32_t a = __float_as_uint(s[2 * G + (d >> 1)][2 * (d & 1)]) | 1u;
+            const uint32_t b = __float_as_uint(s[2 * G + (d >> 1)][2 * (d & 1) + 1]) | 1u;
+            hi4[d] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            lo4[d] = pack_bf16x2(__uint_as_float(a) - __uint_as_float(a & 0xFFFF0000u),
+                                 __uint_as_float(b) - __uint_as_float(b & 0xFFFF0000u));
         }
         typename VRow<B16>::type vv[8];
 #pragma unroll

@@ -297,9 +297,11 @@ int fp8kv_prefill_attn_varlen_bf16(const void* q, int64_t q_row_stride,
  *   - Block-table entries of blocks without a visible key are never used, whatever they hold, so blocks that the
  *     window has left can be given back.
  *   - Rows that see nothing are zeros: seq_lens[s] <= 0, and rows of negative position (seq_lens[s] < qlen_s).
- *   - Keys that a row does not see do not reach it, whatever they hold (a NaN or an infinity included); a
- *     non-finite element of a key that it sees reaches that element of its output.
- * Decode weighs V in two bf16 parts (error 2^-17 of a weight); prefill rounds the weights to bf16 and divides by
+ *   - Keys that a row does not see do not reach it, whatever they hold (a NaN or an infinity included).  Of a key that
+ *     it sees, a non-finite element of V reaches that element of its output (an infinity as itself, unless its weight
+ *     is next to nothing: below 2^-100 of the largest it may be NaN), and a NaN score, from a key, a query or a scale,
+ *     makes the row NaN.
+ * Decode weighs V in two bf16 parts (error 2^-16 of a weight); prefill rounds the weights to bf16 and divides by
  * the sum of the rounded ones.
  * No counterpart in the reference, whose hook leaves such layers to stock vLLM (vllm-fp8kv/fp8kv_override.py:50-64). */
 /* num_splits of the decode calls below and of fp8kv_decode_attn_blk for a batch whose longest context is max_seq_len (0

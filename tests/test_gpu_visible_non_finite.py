@@ -92,3 +92,23 @@ def test_prefill_nan_in_queries(kind, HQ, HKV):
         c["q"][row, head, element] = value
         want[row, head] = NAN
     _agrees(_run(c, "prefill").double(), want, _tolerance(c, "prefill", want, *bounds))
+
+
+@pytest.mark.parametrize("cut", CUTS.values(), ids=CUTS.keys())
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 20)])
+def test_decode_infinite_values(cut, window, sinks):
+    """An infinity in V is that infinity in its element of the output; two of either sign are NaN."""
+    c = _case("bf16", LENS, 8, 2, 16, window, sinks, seed=35, spread=0.3)
+    want, *bounds = _oracle(c)
+    tol = _tolerance(c, "decode", want, *bounds)
+    for value in (INF, -INF):
+        bad = dict(c)
+        _plant(bad, 0, 640, 1, D + 40, value)
+        _plant(bad, 0, 12, 0, D + 3, value)
+        _plant(bad, 1, 40, 0, D + 127, value)
+        _plant(bad, 2, 300, 1, D, value)
+        _plant(bad, 2, 180, 1, D, -value)
+        then = want.clone()
+        then[0, 4:, 40] = then[0, :4, 3] = then[1, :4, 127] = value
+        then[2, 4:, 0] = NAN
+        _agrees(_run(bad, "decode", **cut).double(), then, tol)
