@@ -25,7 +25,8 @@
 //     that divides the result is that of the ROUNDED weights, so that they add up to one (v_dot2_f32_bf16 with ones:
 //     four instructions for a row-set's eight weights).
 //   * a masked key's V must not reach a row through 0 * NaN: on masked tiles that hold a non-finite V
-//     (one test of the raw words), it is zeroed for the product and added afterwards to the rows that see it.
+//     (one test of the raw words, with block scales of the range that each group's scale leaves its codes), it is zeroed
+//     for the product and added afterwards to the rows that see it.
 // Measured in a graph: 2048 block-scaled tokens after 2048, 24 / 4 heads, 92.9 us (832 Tflop/s of visible work; a large bf16
 // product 1117), 4096 e4m3 tokens with a window of 1024 64.3, six block-scaled prompts of 37..900 46.5, five bf16
 // prompts of 100..1500 with a window of 512, 32 / 8 heads, 61.9.  The matrix units are busy 36 % of the time, the vector units
@@ -56,17 +57,26 @@ __device__ __forceinline__ f32x4_t score_mfma(const v8i& k, const v8i& q, f32x4_
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, q, c, 0, 0, 2 * KG, (int)scales, LO ? 1 : 0, qs);
 }
 
-// Any non-finite element among the e4m3 codes (bf16 values) of a word.
+// Any non-finite element among the e4m3 codes (bf16 values) of a word: its field's top bit.  `past` (past_range) lets codes
+// count whose value leaves the range of 32 bits with their group's scale.
+constexpr uint32_t kNanCodes = 0x01010101u;           // NaN alone
 template <bool B16>
-__device__ __forceinline__ uint32_t non_finite(uint32_t w)
+__device__ __forceinline__ uint32_t non_finite(uint32_t w, uint32_t past = kNanCodes)
 {
-    return B16 ? ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u : ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+    return B16 ? ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u : ((w & 0x7F7F7F7Fu) + past) & 0x80808080u;
+}
+// What lifts the magnitude of such a code to its field's top bit.  |code| 2^(byte - 127) >= 2^128, which the widening to bf16
+// makes infinite, from byte 247 on (448 * 2^119 is below): the least such code is 2^(255 - byte), whose bits are
+// (262 - byte) << 3.
+__device__ __forceinline__ uint32_t past_range(uint32_t byte)
+{
+    return byte < 247u ? kNanCodes : (0x80u - ((262u - byte) << 3)) * 0x01010101u;
 }
 // The word with its non-finite elements zeroed.
 template <bool B16>
-__device__ __forceinline__ uint32_t finite_only(uint32_t w)
+__device__ __forceinline__ uint32_t finite_only(uint32_t w, uint32_t past = kNanCodes)
 {
-    const uint32_t bad = non_finite<B16>(w);          // the top bit of each bad element's field
+    const uint32_t bad = non_finite<B16>(w, past);    // the top bit of each bad element's field
     const uint32_t mask = B16 ? (bad << 1) - (bad >> 15) : (bad << 1) - (bad >> 7);
     return w & ~mask;
 }
@@ -439,6 +449,7 @@ prefill_visible_kernel(VisibleParams P)
                 [[maybe_unused]] u32x4_t vf[8];
                 [[maybe_unused]] u32x2_t vr[8];
                 [[maybe_unused]] float vsc[2] = {1.f, 1.f};
+                [[maybe_unused]] uint32_t past[2] = {kNanCodes, kNanCodes};       // of the tile's two groups
                 // V^T fragments 4 w .. 4 w + 3 (d = 8c + 4w ..) from word w of the raw rows, as v_fragments
                 auto widen = [&](int w) {
 #pragma unroll
@@ -477,14 +488,20 @@ prefill_visible_kernel(VisibleParams P)
                     if (masked) {
                         uint32_t bad = 0;
                         asm volatile("" : "+v"(bad));  // a branch: nothing of the test runs on other tiles
+                        if constexpr (SC) {
+                            const uint32_t u = __builtin_amdgcn_readfirstlane(scales);
+                            past[0] = past_range((u >> 8) & 0xFFu);
+                            past[1] = past_range(u >> 24);
+                        }
 #pragma unroll
-                        for (int jj = 0; jj < 8; ++jj) bad |= non_finite<false>(vr[jj][0]) | non_finite<false>(vr[jj][1]);
+                        for (int jj = 0; jj < 8; ++jj)
+                            bad |= non_finite<false>(vr[jj][0], past[jj >> 2]) | non_finite<false>(vr[jj][1], past[jj >> 2]);
                         poisoned = __any(bad != 0);
                         if (poisoned) {
 #pragma unroll
                             for (int jj = 0; jj < 8; ++jj) {
-                                vr[jj][0] = finite_only<false>(vr[jj][0]);
-                                vr[jj][1] = finite_only<false>(vr[jj][1]);
+                                vr[jj][0] = finite_only<false>(vr[jj][0], past[jj >> 2]);
+                                vr[jj][1] = finite_only<false>(vr[jj][1], past[jj >> 2]);
                             }
                         }
                     }
@@ -623,7 +640,8 @@ prefill_visible_kernel(VisibleParams P)
                                 const unsigned char* src = B16 ? buf + TILE / 2 + b16_slot(row, 4 * part + e)
                                     : buf + TILE / 2 + (row >> 3) * 1024 + 16 * v_slot(row & 7, 2 * part + (e >> 1)) + 8 * (e & 1);
                                 const uint32_t w = reinterpret_cast<const uint32_t*>(src)[d];
-                                if (!__any(non_finite<B16>(w) != 0)) continue;
+                                const uint32_t bad = non_finite<B16>(w, past[row >> 4]);
+                                if (!__any(bad != 0)) continue;
 #pragma unroll
                                 for (int j = 0; j < RS; ++j) {
                                     const int qpos = q0 + tok0 + 16 * my_block[j] + (ln & 15);
@@ -636,7 +654,9 @@ prefill_visible_kernel(VisibleParams P)
                                             const uint32_t bits = h ? w & 0xFFFF0000u : w << 16;
                                             x = (bits & 0x7F800000u) == 0x7F800000u ? __uint_as_float(bits) : 0.f;
                                         } else {
-                                            x = ((w >> (8 * h)) & 0x7Fu) == 0x7Fu ? __builtin_nanf("") : 0.f;
+                                            const uint32_t code = w >> (8 * h);
+                                            const float inf = code & 0x80u ? neg_inf() : -neg_inf();
+                                            x = (code & 0x7Fu) == 0x7Fu ? __builtin_nanf("") : bad >> (8 * h) & 0x80u ? inf : 0.f;
                                         }
                                         o[j][per * d + h][e] += sees ? x : 0.f;
                                     }

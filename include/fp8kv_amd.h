@@ -302,7 +302,8 @@ int fp8kv_prefill_attn_varlen_bf16(const void* q, int64_t q_row_stride,
  *     is next to nothing: below 2^-100 of the largest it may be NaN), and a NaN score, from a key, a query or a scale,
  *     makes the row NaN.
  * Decode weighs V in two bf16 parts (error 2^-16 of a weight); prefill rounds the weights to bf16 and divides by
- * the sum of the rounded ones.
+ * the sum of the rounded ones.  Sums are formed in 32 bits, prefill's with weights of up to 2^8: where |V| comes near
+ * 2^100 they may overflow.
  * No counterpart in the reference, whose hook leaves such layers to stock vLLM (vllm-fp8kv/fp8kv_override.py:50-64). */
 /* num_splits of the decode calls below and of fp8kv_decode_attn_blk for a batch whose longest context is max_seq_len (0
  * with a window: not known; >= 2^30: not known).  bf16: whether the caches are.  At most 256. */
@@ -360,8 +361,9 @@ int fp8kv_prefill_attn_window_bf16(const void* q, int64_t q_row_stride,
  * Attention over a block-scaled cache (fp8kv_rope_append_blk): e4m3 codes with one power-of-two scale per 16
  * tokens, kv head and tensor,
  *   K_t = code * 2^(b_K - 127), V_t = code * 2^(b_V - 127), b = kv_scales[block][slot / 16][kv head],
- * kv_scales uint8 [blocks, block_size / 16, num_kv_heads, 2] contiguous, 2-byte aligned, bytes in [1, 254].  With
- * window and sinks as above (0, 0: whole causal contexts); everything else, the guarantees too, as there.
+ * kv_scales uint8 [blocks, block_size / 16, num_kv_heads, 2] contiguous, 2-byte aligned, bytes in [1, 254].  A V of
+ * 2^128 or more (bytes from 247 on) counts as infinite.  With window and sinks as above (0, 0: whole causal contexts);
+ * everything else, the guarantees too, as there.
  * No counterpart in the reference. */
 int fp8kv_decode_attn_blk(const void* q, int64_t q_row_stride,
                           const void* k_cache, const void* v_cache,

@@ -112,3 +112,39 @@ def test_decode_infinite_values(cut, window, sinks):
         then[0, 4:, 40] = then[0, :4, 3] = then[1, :4, 127] = value
         then[2, 4:, 0] = NAN
         _agrees(_run(bad, "decode", **cut).double(), then, tol)
+
+
+# e4m3 codes whose value times 2^(byte - 127) is 2^128 or more, the least of them first
+TOO_LARGE = {247: (0x78, 0x7E), 248: (0x70, 0xF0, 0x7E), 250: (0x60, 0xFE), 254: (0x40, 0xC0, 0x7E)}
+
+
+@pytest.mark.parametrize("byte", TOO_LARGE)
+def test_values_past_32_bits_count_as_infinite(byte):
+    """Elements of a block-scaled V that leave the range of 32 bits: infinite for the rows that see them, nothing for the
+    others; the largest that stays within it is like any other."""
+    for form, lens in (("prefill", [(0, 200)]), ("decode", [(199, 1)])):
+        c = _case("blk", lens, 6, 1, 16, 48, 4, seed=36)
+        token = 70 if form == "prefill" else 170
+        c["pool"], c["scales"] = c["pool"].clone(), c["scales"].clone()
+        block = int(c["table"][0, token // 16])
+        c["pool"][block, :, :, D:] = 0
+        c["scales"][block, :, :, 1] = byte
+        want, *bounds = _oracle(c)
+        tol = _tolerance(c, form, want, *bounds)
+        first = 200 - c["q"].shape[0]
+        t = torch.arange(first, 200)
+        sees = (t >= token) & (t < token + 48)
+        assert sees.any()
+        for code in TOO_LARGE[byte]:
+            bad = dict(c)
+            _plant(bad, 0, token, 0, D + 40, code)
+            _plant(bad, 0, token, 0, D + 41, 0x7F)
+            then = want.clone()
+            then[sees, :, 40] = -INF if code & 0x80 else INF
+            then[sees, :, 41] = NAN
+            _agrees(_run(bad, form).double(), then, tol)
+        # the largest finite one, where only rows that do not see it are looked at, and finite for those that do
+        bad = dict(c)
+        _plant(bad, 0, token, 0, D + 40, (TOO_LARGE[byte][0] & 0x7F) - 1)
+        got = _run(bad, form).double()
+        assert ((got - want).abs() <= tol)[~sees].all() and not got[sees].isnan().any()
