@@ -183,6 +183,8 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
     // them; later reads of these fields reuse the loaded values.
     int seqlen = seq_lens[blockIdx.z];
     int qtok = qsl[blockIdx.z];
+    [[maybe_unused]] int next_tok = 0;
+    if constexpr (VISIBLE && !PARTS) next_tok = qsl[blockIdx.z + 1];
     int nsplit = P.nsplit;
     const int32_t* bt = P.bt;
     int64_t bt_stride = P.bt_stride;
@@ -215,6 +217,10 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
         seqlen = part.len;
         qtok = ((const_i32_t*)qsl)[seq];
     }
+    // A sequence that owns no row of q (padding) has no output: nothing is read or written for it.
+    if constexpr (VISIBLE && !PARTS) {
+        if (next_tok == qtok) return;
+    }
     // One segment: a split of one sequence, or what a part holds of one of its sequences.
     for (;;) {
         int tid = threadIdx.x;
@@ -228,14 +234,25 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
         int64_t rec0;                                      // where the split records of this (sequence, kv head) start,
         int nrec;                                          // and how many there are
         [[maybe_unused]] Walk walk;
-        [[maybe_unused]] int next_len = 0, next_tok = 0, groups = 0;
+        [[maybe_unused]] int next_len = 0, groups = 0;
         if constexpr (VISIBLE) {
             walk = make_walk(seqlen, P.window, P.sinks);
         }
+        // On to the part's next sequence, if it has one.
+        [[maybe_unused]] auto advance = [&]() -> bool {
+            if constexpr (PARTS) {
+                part.base += groups;
+                ++seq;
+                seqlen = next_len;
+                qtok = next_tok;
+                return part.base < part.start + part.size && seq < P.ns;
+            }
+            return false;
+        };
         if constexpr (PARTS) {
             const int next = seq + 1 < P.ns ? seq + 1 : seq;
             next_len = ((const_i32_t*)seq_lens)[next];
-            next_tok = ((const_i32_t*)qsl)[next];
+            next_tok = ((const_i32_t*)qsl)[seq + 1];
             groups = walk_groups(walk.nv);
             const int w = blockIdx.x, end = part.start + part.size;
             lo = part.start > part.base ? 16 * (part.start - part.base) : 0;
@@ -246,6 +263,10 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
             nrec = past - first + 1;
             // A record's place counts the parts and the sequences before it.
             rec0 = (int64_t)kh * (P.parts + P.ns) + first + seq;
+            if (next_tok == qtok) {                        // owns no row, as above
+                if (!advance()) return;
+                continue;
+            }
         } else {
             int tokens = seqlen;
             if constexpr (VISIBLE) tokens = walk.nv;
@@ -509,11 +530,7 @@ __device__ __forceinline__ void decode_body(const int32_t* __restrict__ seq_lens
         };
         finish();
         if constexpr (PARTS) {
-            part.base += groups;
-            ++seq;
-            if (part.base >= part.start + part.size || seq >= P.ns) return;
-            seqlen = next_len;
-            qtok = next_tok;
+            if (!advance()) return;
             __syncthreads();                               // the next segment's states go where this one's were read
         } else {
             return;

@@ -531,7 +531,8 @@ def decode_attention_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     t > p - window and the first ``sinks`` ones (window 0: all).  Caches e4m3 with per-tensor scales, or bf16.
     ``out`` has a row for every row of ``q`` (here and in the three calls below).
 
-    Only the visible keys are read; block-table entries of blocks that hold none may be anything.  A window bounds
+    Only the visible keys are read; block-table entries of blocks that hold none may be anything.  Sequences that own no
+    row of ``q`` (query_start_loc[s + 1] == query_start_loc[s], as in a padded batch) write none.  A window bounds
     the work, so ``max_seq_len`` is needed only without one (and then read from ``seq_lens``, which synchronises).
     ``scratch`` defaults to a buffer of the current stream's, or of the graph's under capture, so that calls on two
     streams and replays may run at once; one that is given is for one call at a time."""

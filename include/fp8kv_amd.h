@@ -297,6 +297,8 @@ int fp8kv_prefill_attn_varlen_bf16(const void* q, int64_t q_row_stride,
  *   - Block-table entries of blocks without a visible key are never used, whatever they hold, so blocks that the
  *     window has left can be given back.
  *   - Rows that see nothing are zeros: seq_lens[s] <= 0, and rows of negative position (seq_lens[s] < qlen_s).
+ *   - Sequences that own no row (query_start_loc[s + 1] == query_start_loc[s]: a padded batch) write none, and none of
+ *     their blocks is read; seq_lens[s] has to be a length all the same.
  *   - Keys that a row does not see do not reach it, whatever they hold (a NaN or an infinity included).  Of a key that
  *     it sees, a non-finite element of V reaches that element of its output (an infinity as itself, unless its weight
  *     is next to nothing: below 2^-100 of the largest it may be NaN), and a NaN score, from a key, a query or a scale,
