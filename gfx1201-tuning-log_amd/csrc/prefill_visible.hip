@@ -449,7 +449,11 @@ prefill_visible_kernel(VisibleParams P)
                 [[maybe_unused]] u32x4_t vf[8];
                 [[maybe_unused]] u32x2_t vr[8];
                 [[maybe_unused]] float vsc[2] = {1.f, 1.f};
-                [[maybe_unused]] uint32_t past[2] = {kNanCodes, kNanCodes};       // of the tile's two groups
+                // past_range of group g of the tile
+                [[maybe_unused]] auto past_of = [&](int g) {
+                    if constexpr (SC) return past_range((uint32_t)__builtin_amdgcn_readfirstlane(lds_scales[i & 1][tw][g]) >> 8);
+                    else return kNanCodes;
+                };
                 // V^T fragments 4 w .. 4 w + 3 (d = 8c + 4w ..) from word w of the raw rows, as v_fragments
                 auto widen = [&](int w) {
 #pragma unroll
@@ -473,9 +477,11 @@ prefill_visible_kernel(VisibleParams P)
                                        (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
                     }
                     uint32_t scales = 127 | 127 << 16;
+                    [[maybe_unused]] uint32_t tile_scales = 0;
                     if constexpr (SC) {
                         scales = *reinterpret_cast<const uint32_t*>(lds_scales[i & 1][tw]);
                         const uint32_t u = __builtin_amdgcn_readfirstlane(scales);
+                        tile_scales = u;
                         vsc[0] = __uint_as_float((u & 0xFF00u) << 15);         // bytes 1 .. 254 are exponents as they are
                         vsc[1] = __uint_as_float((u & 0xFF000000u) >> 1);
                     }
@@ -488,16 +494,12 @@ prefill_visible_kernel(VisibleParams P)
                     if (masked) {
                         uint32_t bad = 0;
                         asm volatile("" : "+v"(bad));  // a branch: nothing of the test runs on other tiles
-                        if constexpr (SC) {
-                            const uint32_t u = __builtin_amdgcn_readfirstlane(scales);
-                            past[0] = past_range((u >> 8) & 0xFFu);
-                            past[1] = past_range(u >> 24);
-                        }
 #pragma unroll
-                        for (int jj = 0; jj < 8; ++jj)
-                            bad |= non_finite<false>(vr[jj][0], past[jj >> 2]) | non_finite<false>(vr[jj][1], past[jj >> 2]);
+                        for (int jj = 0; jj < 8; ++jj) bad |= non_finite<false>(vr[jj][0]) | non_finite<false>(vr[jj][1]);
                         poisoned = __any(bad != 0);
+                        if constexpr (SC) poisoned |= (tile_scales & 0xFF00u) >= 247u << 8 || tile_scales >> 24 >= 247u;
                         if (poisoned) {
+                            const uint32_t past[2] = {past_of(0), past_of(1)};
 #pragma unroll
                             for (int jj = 0; jj < 8; ++jj) {
                                 vr[jj][0] = finite_only<false>(vr[jj][0], past[jj >> 2]);
@@ -633,6 +635,7 @@ prefill_visible_kernel(VisibleParams P)
                     const int part = ln >> 4;
                     for (int row = 0; row < kBN; ++row) {
                         const int key = k0 + row;
+                        const uint32_t past = past_of(row >> 4);
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -640,7 +643,7 @@ prefill_visible_kernel(VisibleParams P)
                                 const unsigned char* src = B16 ? buf + TILE / 2 + b16_slot(row, 4 * part + e)
                                     : buf + TILE / 2 + (row >> 3) * 1024 + 16 * v_slot(row & 7, 2 * part + (e >> 1)) + 8 * (e & 1);
                                 const uint32_t w = reinterpret_cast<const uint32_t*>(src)[d];
-                                const uint32_t bad = non_finite<B16>(w, past[row >> 4]);
+                                const uint32_t bad = non_finite<B16>(w, past);
                                 if (!__any(bad != 0)) continue;
 #pragma unroll
                                 for (int j = 0; j < RS; ++j) {
