@@ -23,14 +23,16 @@
 //     through LDS.
 //   * the weights are rounded to bf16 for P.V, which has the range for any score and any block scale, and the sum
 //     that divides the result is that of the ROUNDED weights, so that they add up to one (v_dot2_f32_bf16 with ones:
-//     four instructions for a row-set's eight weights).
+//     four instructions for a row-set's eight weights).  Outputs are 0.0018 of their norm off those of 64 bits, with weights
+//     in 32 bits 0.0016 (most of it their own rounding to bf16); a second part of each weight would double P.V's products.
 //   * a masked key's V must not reach a row through 0 * NaN: on masked tiles that hold a non-finite V
 //     (one test of the raw words, with block scales of the range that each group's scale leaves its codes), it is zeroed
 //     for the product and added afterwards to the rows that see it.
-// Measured in a graph: 2048 block-scaled tokens after 2048, 24 / 4 heads, 92.9 us (832 Tflop/s of visible work; a large bf16
-// product 1117), 4096 e4m3 tokens with a window of 1024 64.3, six block-scaled prompts of 37..900 46.5, five bf16
-// prompts of 100..1500 with a window of 512, 32 / 8 heads, 61.9.  The matrix units are busy 36 % of the time, the vector units
-// 52 %.  Without the exponentials the first would take 10 us less, without the second part of Q 7, without widening V 7.
+// Measured in a graph: 2048 block-scaled tokens after 2048, 24 / 4 heads, 91.6 us (844 Tflop/s of visible work; a large bf16
+// product 1117), 4096 e4m3 tokens with a window of 1024 63.6, six block-scaled prompts of 37..900 47.0, five bf16
+// prompts of 100..1500 with a window of 512, 32 / 8 heads, 62.4.  The matrix units are busy 36 % of the time, the vector units
+// 53 % (the six prompts: 25 and 50, the five: 26 and 51).  At an earlier step, when the first took 104 us, it was 10
+// faster without the exponentials, 7 without the second part of Q and 7 without widening V.
 #include "fp8kv_common.h"
 #include "fp8kv_status.h"
 #include "fp8kv_diag.h"
@@ -747,7 +749,8 @@ prefill_visible_kernel(VisibleParams P)
 // keys, start and end once, and leave fewer partial states to merge; fewer blocks split the keys over more waves, so the
 // GPU is full with fewer tokens.  The shape follows from the time that each would take, in us, fitted to 100 batches
 // (1 to 16 sequences of 100..4000, GQA 4 to 10, either cache width) at every shape; the one taken is 1.1 % slower than
-// the best on average, 32 % at most:
+// the best on average, 32 % at most.  Outside of them, 24 batches of 300..4000 each: GQA 1 7.6 % on average and 40 % at most
+// (16 of 30..300: 42.0 us in blocks of 256 tokens, 30.0 in 384), 2 and 3 3 % and 13 %, 11 to 16 1.5 % and 14 %.  The terms:
 //   a workgroup   9.5 (three row-sets a wave: 9.6), and per key tile 0.2 (bf16: 0.3) for its copies and 0.65 (two row-sets
 //                 a wave) or 1.2 (three) times the filled part of its eight waves, where a wave without rows still costs
 //                 three quarters;
