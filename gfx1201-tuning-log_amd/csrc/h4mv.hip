@@ -497,7 +497,7 @@ h4mv_stream_kernel(const uint8_t* __restrict__ W, const uint8_t* __restrict__ St
 //     meet once, at the end, and wave w adds the partials of tiles w, w + nw, ... in wave order
 //     (a fixed order: the result does not depend on timing) and writes them through store_tile.
 // Activation traffic is then one step of X per wave and launch instead of per tile.  Measured
-// (cfg1 and configs[4] gate/up, M = 1 .. 8): the marginal stream rate is the same at every M and
+// (K = 4096, N = 28672 and K = 3584, N = 37888, M = 1 .. 8): the marginal stream rate is the same at every M and
 // higher than the streaming kernel's, but the fixed cost per launch is about 1 us higher, so the
 // planner takes it from M = 3 on (gate/up M = 8: 20.9 -> 15.7 us, cfg1 M = 8: 14.8 -> 13.6 us;
 // M = 2 and 1 stay faster on the streaming kernel).

@@ -7,7 +7,7 @@
 //
 // gfx950 design: a 64 x 64 byte tile per workgroup, read along N and written along K/32 through
 // LDS (row pitch 68 bytes to spread the column reads of the write phase over the banks); each
-// thread moves 4 bytes per step.  It runs once per weight (3.7 MB at configs[1]), so it is written for
+// thread moves 4 bytes per step.  It runs once per weight (3.7 MB at K = 4096, N = 28672), so it is written for
 // plain coalescing rather than peak bandwidth.
 #include "fp8kv_common.h"
 #include "fp8kv_status.h"

@@ -18,8 +18,8 @@
 // 8 that hold whole pairs of either kind: (8 u, 8 u + R / 2) where halves are paired, else
 // (16 u, 16 u + 8); each piece is one 16-byte load, and both table rows are read at 8 u.  Measured in a graph:
 // 4096 tokens of 28 + 4 heads, bf16, 15.9 us (4.8 TB/s; a large copy 5.5), six prompts of 37..900, block-scaled, 10.7
-// (4.2 TB/s), one token 3.3, 64 tokens block-scaled 4.7, 2048 tokens of 24 + 4 heads, e4m3, 9.8 (3.3 TB/s).  Four heads per thread, which read the table once, are no
-// faster (15.6 and 10.9) and 7.5 for one token.
+// (4.2 TB/s), one token 3.3, 64 tokens block-scaled 4.7, 2048 tokens of 24 + 4 heads, e4m3, 9.8 (3.3 TB/s).  Four heads
+// per thread, which read the table once, are no faster (15.6 and 10.9) and 7.5 for one token.
 #include "fp8kv_common.h"
 #include "fp8kv_status.h"
 #include "e4m3_store.h"

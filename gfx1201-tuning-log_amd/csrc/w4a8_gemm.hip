@@ -43,7 +43,7 @@ constexpr int kBN = 128, kBM = 128;
 // registers capped for two waves per SIMD, 3-step ring; 5: as 4 with a 2-step ring (51 KB of
 // LDS, so up to three workgroups share a CU); 6 / 7: as 5 with 8 x 4 / 4 x 8 MFMA tiles per wave;
 // 8: 8 waves of 8 x 4 tiles (256 x 256 per workgroup, 3-step ring, 150 KB of LDS).  Measured on
-// the configs[4] linears at M = 2048: 6 ~1.22-1.69 PFLOP/s, 5 ~1.27-1.41, 8 ~0.88-1.67 (only
+// the four linears of a layer (hidden 3584, gate/up 37888) at M = 2048: 6 ~1.22-1.69 PFLOP/s, 5 ~1.27-1.41, 8 ~0.88-1.67 (only
 // gate/up fills the GPU), 7 ~1.05-1.27, 4 ~1.33, 0 ~1.01, 1 ~0.40.
 // Default (-1): the K-splitting kernel where its tiles fit one round (slice_shape); else variant 6 (the
 // 8 x 4 wave tile, 256 x 128 per workgroup) when its grid has more tiles than the GPU has CUs, else 128 x 128
@@ -1000,7 +1000,7 @@ constexpr int kLdsPerCu = 160 * 1024;
 // that, among the splits under which an XCD's activation share is reused from its L2: either all
 // the XCD's tiles run in one round of resident workgroups (the tiles of a round stream K together)
 // or the share fits half an L2 (it then survives the weight tiles streamed between rounds).
-// Measured at the configs[4] linears, M = 2048, against the token-block split as far as the
+// Measured at the same linears, M = 2048, against the token-block split as far as the
 // count allows (bytes fetched into the L2s, FETCH_SIZE): qkv 70 -> 46 MB, o 53 -> 36 MB, gate/up
 // 667 -> 419 MB, down 332 -> 226 MB; kernel time 1-4 % lower (qkv 42.3 -> 40.5 us, down 193.9 ->
 // 188.4 us).

@@ -77,8 +77,8 @@ def _make_cache(nb: int, pblk: int, hkv: int, d: int, g: torch.Generator, layout
 
 def engine_pool_amax(nb: int, hkv: int, pblk: int, d: int, generator: torch.Generator,
                      device) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """An engine-layout fp8 KV pool [nb, hkv, pblk, 2d] (K | V) built on `device` the way
-    BASELINE.json configs[0] specifies the cache: K and V ~ N(0,1), each quantised to e4m3 with a
+    """An engine-layout fp8 KV pool [nb, hkv, pblk, 2d] (K | V) built on `device` like
+    the cache of the one-sequence decode workload (512 tokens): K and V ~ N(0,1), each quantised to e4m3 with a
     per-tensor scale amax / 448.  Returns (pool, k_scale, v_scale), the scales as fp32 [1]
     device tensors (the form the attention hooks pass)."""
     pool = torch.empty(nb, hkv, pblk, 2 * d, dtype=torch.uint8, device=device)
