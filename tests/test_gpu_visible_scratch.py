@@ -136,3 +136,32 @@ def test_capture_numbers():
         assert a == b != 0
         seen.append(a)
     assert len(set(seen)) == 3 and lib.fp8kv_stream_capture(side.cuda_stream) == 0
+
+
+def test_graphs_come_and_go():
+    """Graphs that are dropped, one that stays, a shared pool, and eager calls between: a capture's scratch is its graph's."""
+    batches = _batches()
+    want = [b.alone() for b in batches]
+    kept = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(kept):
+        kept_out = [b.run(torch.empty_like(b.q)) for b in batches]          # each needs another size of scratch
+    for i in range(6):
+        graph = torch.cuda.CUDAGraph()
+        b = i % 3
+        with torch.cuda.graph(graph, pool=kept.pool() if i % 2 else None):
+            out = batches[b].run(torch.empty_like(batches[b].q))
+            wide = torch.full((1 << 20,), 3.0, device=DEV)                  # other memory of the graph's
+            again = batches[b].run(torch.empty_like(batches[b].q))
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[b]) and torch.equal(again, want[b]) and (wide == 3).all()
+            assert torch.equal(batches[(b + 1) % 3].run(), want[(b + 1) % 3])
+        del graph, out, wide, again
+        if i % 2:
+            torch.cuda.empty_cache()
+        for o in kept_out:
+            o.fill_(7.0)
+        kept.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(kept_out, want)), i
